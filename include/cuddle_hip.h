@@ -518,6 +518,79 @@ cuddle_status cuddle_sharded_search_batch(cuddle_index *shard, cuddle_comm *comm
                                           uint32_t flags, uint64_t *d_out_ids, float *d_out_dist,
                                           uint32_t *d_out_count, void *stream);
 
+/* ---- embedding table: 4-bit rows, row lookup, its gradient --------------------------------------
+ * No counterpart in the reference, whose codes are 1-bit and whose rows are fetched one at a time
+ * (MmapVectorStore::get, src/storage/mmap.rs:106-115). Conventions of these calls: device pointers of
+ * `device_id` (the caller's current device is left as it was), everything enqueued on `stream`, nothing
+ * allocated, nothing copied to the host, nothing but kernels, so all of them may be recorded into a graph.
+ * Work space is the caller's ([256-byte aligned], its size from the *_workspace call of the same sizes); it
+ * holds nothing between calls, and two calls may share it only if they cannot overlap. Results are the same
+ * bits from run to run. Arguments are checked before anything is enqueued. Row strides are in elements.
+ * An id outside [0, rows) (any negative one: padding) names no row: a lookup gives zeros for it, a gradient
+ * leaves it out. dim <= 32768; fewer than 2^32 - 1 rows. */
+typedef enum cuddle_type { CUDDLE_TYPE_F32 = 0, CUDDLE_TYPE_F16 = 1, CUDDLE_TYPE_BF16 = 2 } cuddle_type;
+
+/* 4-bit rows. Components are cut into groups of `group` (32, 64 or 128; the last may be shorter): scale
+ * s = bf16(max|x| / 7), code c = rint(x / s) with halves to even, clamped to -7..7 (0 where s is 0); the
+ * row stands for s * c. A group with a NaN or an infinity has s = NaN and codes 0: such a row decodes to
+ * NaN there, and its distances are NaN.
+ *   codes  : blocks of 16 rows x 64 components, 512 bytes each, the blocks of 16 rows one after the
+ *            other; in a block row r has 32 bytes, byte 8h + i (h < 4, i < 8) holding component 8h + i in
+ *            its low and 32 + 8h + i in its high nibble, two's complement; components past dim are 0, rows
+ *            past n arbitrary. cuddle_int4_sizes gives the bytes. 16-byte aligned.
+ *   scales : [n][scale_stride] bf16, scale_stride = ceil(dim / group) rounded up to an even number; 4-byte aligned
+ *   sqnorm : [n] f64, |row|^2 of what the row stands for; distances use it (NULL is allowed for DOT and lookups) */
+typedef struct cuddle_int4_rows {
+    void *codes;
+    void *scales;
+    void *sqnorm;
+    uint64_t n;
+    uint32_t dim;
+    uint32_t group;
+} cuddle_int4_rows;
+
+/* Bytes of `codes` and elements between two rows of `scales`. */
+cuddle_status cuddle_int4_sizes(uint64_t n, uint32_t dim, uint32_t group, uint64_t *code_bytes,
+                                uint32_t *scale_stride);
+/* Encodes `count` rows of f32, f16 or bf16 into rows [first_row, first_row + count); others are left alone. */
+cuddle_status cuddle_int4_encode_device(const cuddle_int4_rows *rows, uint64_t first_row, uint64_t count,
+                                        const void *d_vectors, uint32_t type, uint64_t row_stride,
+                                        int device_id, void *stream);
+/* d_out [n_ids][dim] of out_type = scale * row ids[t]. d_ids: int32 or int64 (id_bits 32 or 64), or NULL for
+ * rows 0 .. n_ids - 1. One rounding to f32 for the product with `scale`, one to out_type. */
+cuddle_status cuddle_int4_lookup_device(const cuddle_int4_rows *rows, const void *d_ids, uint32_t id_bits,
+                                        uint64_t n_ids, float scale, uint32_t out_type, void *d_out,
+                                        int device_id, void *stream);
+/* Work space of the two calls below: k = 0 for distances, the search's k otherwise (k <= 1024). */
+cuddle_status cuddle_int4_workspace(uint64_t n, uint32_t dim, uint32_t n_queries, uint32_t k, uint64_t *bytes);
+/* d_dist [n_queries][n] f32 = distance(query, row) under `metric` (cuddle_metric) of contiguous f32, f16 or bf16
+ * queries to what the rows stand for. Products are exact up to the queries' fixed point (2^-30 of a query's
+ * largest magnitude), sums are f64, a distance is rounded once. L2 is never below 0. A query with a
+ * non-finite value has distance NaN to every row; COSINE with a zero vector is NaN (0 / 0), as the formula says. */
+cuddle_status cuddle_int4_distances_device(const cuddle_int4_rows *rows, const void *d_queries, uint32_t type,
+                                           uint32_t n_queries, uint32_t metric, float *d_dist, void *d_ws,
+                                           uint64_t ws_bytes, int device_id, void *stream);
+/* The k rows of smallest distance per query, among all rows, in order of (distance, row), NaN after everything:
+ * d_out_ids / d_out_dist [n_queries][k], d_out_count [n_queries] or NULL = min(k, n). Unused slots hold
+ * UINT64_MAX and +inf, as cuddle_search_batch leaves them. */
+cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows, const void *d_queries, uint32_t type,
+                                        uint32_t n_queries, uint32_t k, uint32_t metric, uint64_t *d_out_ids,
+                                        float *d_out_dist, uint32_t *d_out_count, void *d_ws,
+                                        uint64_t ws_bytes, int device_id, void *stream);
+/* d_out [n_ids][dim] = scale * d_table[ids[t]], both of `type`; the product is formed in f32. */
+cuddle_status cuddle_rows_lookup_device(const void *d_table, uint32_t type, uint64_t row_stride,
+                                        uint64_t n_rows, uint32_t dim, const void *d_ids, uint32_t id_bits,
+                                        uint64_t n_ids, float scale, void *d_out, int device_id, void *stream);
+/* The lookup's gradient: d_grad [n_rows][dim] of grad_type, row v = scale * the sum of d_grad_out[t] over the
+ * t with ids[t] == v, summed in f32 in a fixed order and rounded once; rows that no id names become 0. With
+ * CUDDLE_GRAD_ACCUMULATE the sums are added to what d_grad holds and the other rows are not touched. Fewer than 2^31 ids. */
+#define CUDDLE_GRAD_ACCUMULATE 0x1u
+cuddle_status cuddle_rows_grad_workspace(uint64_t n_ids, uint64_t n_rows, uint32_t dim, uint64_t *bytes);
+cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_t type, uint64_t row_stride,
+                                      const void *d_ids, uint32_t id_bits, uint64_t n_ids, float scale,
+                                      uint64_t n_rows, uint32_t dim, uint32_t flags, uint32_t grad_type,
+                                      void *d_grad, void *d_ws, uint64_t ws_bytes, int device_id, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

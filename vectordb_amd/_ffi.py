@@ -39,6 +39,8 @@ SEARCH_ROUTE_GROUPED = 0x8
 SEARCH_ROUTE_SPLIT_FILTER = 0x10
 DESC_DEVICE_ARRAYS = 0x1
 DESC_ADOPT_VECTORS = 0x2
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+GRAD_ACCUMULATE = 0x1
 STAGE_NAMES = ("quantize", "route", "scan", "rerank", "topk", "scan_prep")
 
 
@@ -93,6 +95,19 @@ class Stats(C.Structure):
 
     def as_dict(self):
         return {n: int(getattr(self, n)) for n, _ in self._fields_}
+
+
+class Int4RowsDesc(C.Structure):
+    """struct cuddle_int4_rows."""
+
+    _fields_ = [
+        ("codes", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("sqnorm", C.c_void_p),
+        ("n", C.c_uint64),
+        ("dim", C.c_uint32),
+        ("group", C.c_uint32),
+    ]
 
 
 # Every symbol include/cuddle_hip.h declares: name -> (restype, argtypes)
@@ -151,6 +166,15 @@ SIGNATURES = {
     "cuddle_comm_rank": (_int, [_vp]),
     "cuddle_comm_world": (_int, [_vp]),
     "cuddle_sharded_search_batch": (_int, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp]),
+    "cuddle_int4_sizes": (_int, [_u64, _u32, _u32, C.POINTER(_u64), C.POINTER(_u32)]),
+    "cuddle_int4_encode_device": (_int, [C.POINTER(Int4RowsDesc), _u64, _u64, _vp, _u32, _u64, _int, _vp]),
+    "cuddle_int4_lookup_device": (_int, [C.POINTER(Int4RowsDesc), _vp, _u32, _u64, C.c_float, _u32, _vp, _int, _vp]),
+    "cuddle_int4_workspace": (_int, [_u64, _u32, _u32, _u32, C.POINTER(_u64)]),
+    "cuddle_int4_distances_device": (_int, [C.POINTER(Int4RowsDesc), _vp, _u32, _u32, _u32, _vp, _vp, _u64, _int, _vp]),
+    "cuddle_int4_search_device": (_int, [C.POINTER(Int4RowsDesc), _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _u64, _int, _vp]),
+    "cuddle_rows_lookup_device": (_int, [_vp, _u32, _u64, _u64, _u32, _vp, _u32, _u64, C.c_float, _vp, _int, _vp]),
+    "cuddle_rows_grad_workspace": (_int, [_u64, _u64, _u32, C.POINTER(_u64)]),
+    "cuddle_rows_grad_device": (_int, [_vp, _u32, _u64, _vp, _u32, _u64, C.c_float, _u64, _u32, _u32, _u32, _vp, _vp, _u64, _int, _vp]),
     "cuddle_merge_topk_ordered_device": (_int, [_vp, _vp, _vp, _u32, _u32, _u32, _u64, _vp, _vp, _vp, _vp]),
 }
 

@@ -25,6 +25,7 @@
 #include "cuddle_rabitq.hpp"
 #include "cuddle_rabitq_grouped.hpp"
 #include "cuddle_build.hpp"
+#include "cuddle_rows.hpp"
 
 using namespace cuddle;
 
@@ -2899,3 +2900,393 @@ extern "C" cuddle_status cuddle_merge_topk(const uint64_t *lists_ids, const floa
 }
 
 #include "cuddle_comm.hpp"
+
+// ---------------------------------------------------------------------------------------------
+// embedding table: 4-bit rows, lookup, gradient (kernels in cuddle_rows.hpp)
+// ---------------------------------------------------------------------------------------------
+namespace {
+struct DeviceGuard { // the calls below leave the caller's current device as it was
+    int prev = -1;
+    cuddle_status enter(int device_id) {
+        if (hipGetDevice(&prev) != hipSuccess) {
+            (void)hipGetLastError();
+            prev = -1;
+        }
+        return use_device(device_id);
+    }
+    ~DeviceGuard() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+unsigned grid_for(uint64_t blocks) { return (unsigned)std::min<uint64_t>(std::max<uint64_t>(blocks, 1), 1u << 20); }
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+uint32_t type_size(uint32_t type) { return type == CUDDLE_TYPE_F32 ? 4u : 2u; }
+cuddle_status check_type(uint32_t type) { return type > CUDDLE_TYPE_BF16 ? fail(CUDDLE_ERR_BAD_ARG, "unknown element type %u", type) : CUDDLE_OK; }
+cuddle_status check_group(uint32_t group) {
+    return group != 32 && group != 64 && group != 128 ? fail(CUDDLE_ERR_BAD_ARG, "group must be 32, 64 or 128, not %u", group) : CUDDLE_OK;
+}
+cuddle_status check_dim(uint32_t dim) {
+    if (dim == 0) return fail(CUDDLE_ERR_BAD_ARG, "dim must be >= 1");
+    if (dim > 32768) return fail(CUDDLE_ERR_UNSUPPORTED, "dim %u > 32768", dim);
+    return CUDDLE_OK;
+}
+cuddle_status check_rows(const cuddle_int4_rows *r, bool need_sq) {
+    if (!r) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    ST_TRY(check_dim(r->dim));
+    ST_TRY(check_group(r->group));
+    if (r->n >= 0xFFFFFFFFull) return fail(CUDDLE_ERR_UNSUPPORTED, "%llu rows: fewer than 2^32 - 1", (unsigned long long)r->n);
+    if (r->n && (!r->codes || !r->scales || (need_sq && !r->sqnorm))) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    if (!aligned16(r->codes) || ((uintptr_t)r->scales & 3) || ((uintptr_t)r->sqnorm & 7)) return fail(CUDDLE_ERR_BAD_ARG, "codes, scales and sqnorm need alignments of 16, 4 and 8 bytes");
+    return CUDDLE_OK;
+}
+cuddle_status check_ids(const void *ids, uint32_t id_bits) {
+    if (id_bits != 32 && id_bits != 64) return fail(CUDDLE_ERR_BAD_ARG, "ids have 32 or 64 bits, not %u", id_bits);
+    if ((uintptr_t)ids & (id_bits / 8 - 1)) return fail(CUDDLE_ERR_BAD_ARG, "misaligned ids");
+    return CUDDLE_OK;
+}
+cuddle_status check_elem_align(const void *p, uint32_t type) {
+    return (uintptr_t)p & (type_size(type) - 1) ? fail(CUDDLE_ERR_BAD_ARG, "misaligned rows") : CUDDLE_OK;
+}
+
+// Calls f with a value of the element type.
+template <class F> void with_type(uint32_t type, F f) {
+    if (type == CUDDLE_TYPE_F32) f(float{});
+    else if (type == CUDDLE_TYPE_F16) f(_Float16{});
+    else f(Bf16{});
+}
+template <class F> void with_id(uint32_t bits, F f) {
+    if (bits == 32) f(int32_t{});
+    else f(int64_t{});
+}
+
+constexpr size_t kAlign = 256;
+size_t round_ws(size_t b) { return (b + kAlign - 1) & ~(kAlign - 1); }
+
+// Work space of the distance and search calls: the queries' digits, and for a search the distances of `qc` queries and
+// two selection buffers.
+struct Int4Ws {
+    uint32_t qc = 0; // queries per round
+    size_t dig = 0, info = 0, dist = 0, sel[2] = {0, 0}, bytes = 0;
+};
+constexpr uint64_t kInt4DistBudget = 512ull << 20; // bytes of distances a search holds at a time (one quartet of queries at least)
+constexpr uint64_t kInt4MaxRound = 32768;          // queries per round (the launches' second grid dimension)
+
+Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
+    Int4Ws w;
+    uint64_t qc = std::min<uint64_t>(nq, kInt4MaxRound);
+    if (k) qc = std::min<uint64_t>(qc, std::max<uint64_t>(4, kInt4DistBudget / (std::max<uint64_t>(n, 1) * 4) & ~3ull));
+    w.qc = (uint32_t)qc;
+    const uint64_t quartets = (qc + 3) / 4, parts = (n + kTopChunk - 1) / kTopChunk;
+    size_t at = 0;
+    w.dig = at;
+    at += round_ws(quartets * int4_units(dim) * 1024);
+    w.info = at;
+    at += round_ws(quartets * 4 * sizeof(Int4Query));
+    if (k) {
+        w.dist = at;
+        at += round_ws((size_t)qc * n * 4);
+        if (parts > 1) {
+            w.sel[0] = at;
+            at += round_ws((size_t)qc * parts * k * 8);
+            w.sel[1] = at;
+            at += round_ws((size_t)qc * ((parts * k + kTopChunk - 1) / kTopChunk) * k * 8);
+        }
+    }
+    w.bytes = at;
+    return w;
+}
+
+template <int G>
+void int4_launch_distances(const cuddle_int4_rows *r, const uint8_t *dig, const Int4Query *info, uint32_t nq, uint32_t metric, float *dist, uint64_t dstride,
+                           hipStream_t s) {
+    const uint64_t tiles = (r->n + 15) / 16;
+    constexpr int QT = 1, T = 1;
+    hipLaunchKernelGGL((int4_distance_kernel<G, QT, T>), dim3(grid_for((tiles + 4 * T - 1) / (4 * T)), (nq + 4 * QT - 1) / (4 * QT)), dim3(256), 0, s,
+                       (const uint8_t *)r->codes, (const uint16_t *)r->scales, (const double *)r->sqnorm, r->n, r->dim, dig, info, nq, metric, dist, dstride);
+}
+
+// Distances of queries [q0, q0 + nq) into dist[q][dstride]; the caller has laid out the work space for nq queries.
+cuddle_status int4_distances_round(const cuddle_int4_rows *r, const void *queries, uint32_t type, uint32_t q0, uint32_t nq, uint32_t metric, float *dist,
+                                   uint64_t dstride, uint8_t *ws, const Int4Ws &w, hipStream_t s) {
+    uint8_t *dig = ws + w.dig;
+    Int4Query *info = (Int4Query *)(ws + w.info);
+    const uint32_t units = int4_units(r->dim), padded = (nq + 3) / 4 * 4;
+    with_type(type, [&](auto z) {
+        using T = decltype(z);
+        hipLaunchKernelGGL(int4_query_kernel<T>, dim3(padded), dim3(256), 0, s, (const T *)queries + (uint64_t)q0 * r->dim, nq, r->dim, units, dig, info);
+    });
+    if (r->group == 32) int4_launch_distances<32>(r, dig, info, nq, metric, dist, dstride, s);
+    else if (r->group == 64) int4_launch_distances<64>(r, dig, info, nq, metric, dist, dstride, s);
+    else int4_launch_distances<128>(r, dig, info, nq, metric, dist, dstride, s);
+    HIP_TRY(hipGetLastError());
+    return CUDDLE_OK;
+}
+
+cuddle_status check_query_call(const cuddle_int4_rows *r, const void *queries, uint32_t type, uint32_t nq, uint32_t metric) {
+    if (metric > CUDDLE_METRIC_DOT) return fail(CUDDLE_ERR_BAD_ARG, "unknown metric %u", metric);
+    ST_TRY(check_rows(r, metric != CUDDLE_METRIC_DOT));
+    ST_TRY(check_type(type));
+    if (nq && !queries) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    return check_elem_align(queries, type);
+}
+cuddle_status check_ws(const void *ws, uint64_t have, uint64_t need) {
+    if (need && (!ws || have < need)) return fail(CUDDLE_ERR_BAD_ARG, "work space of %llu bytes needed, %llu given", (unsigned long long)need, (unsigned long long)(ws ? have : 0));
+    if ((uintptr_t)ws & (kAlign - 1)) return fail(CUDDLE_ERR_BAD_ARG, "the work space needs an alignment of %zu bytes", kAlign);
+    return CUDDLE_OK;
+}
+} // namespace
+
+extern "C" cuddle_status cuddle_int4_sizes(uint64_t n, uint32_t dim, uint32_t group, uint64_t *code_bytes, uint32_t *scale_stride) {
+    if (!code_bytes || !scale_stride) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    ST_TRY(check_dim(dim));
+    ST_TRY(check_group(group));
+    if (n >= 0xFFFFFFFFull) return fail(CUDDLE_ERR_UNSUPPORTED, "%llu rows: fewer than 2^32 - 1", (unsigned long long)n);
+    *code_bytes = (n + 15) / 16 * int4_units(dim) * kInt4UnitBytes;
+    *scale_stride = int4_gstride(dim, group);
+    return CUDDLE_OK;
+}
+
+extern "C" cuddle_status cuddle_int4_encode_device(const cuddle_int4_rows *rows, uint64_t first_row, uint64_t count, const void *d_vectors, uint32_t type,
+                                                   uint64_t row_stride, int device_id, void *stream_) {
+    ST_TRY(check_rows(rows, true));
+    ST_TRY(check_type(type));
+    if (count && !d_vectors) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    ST_TRY(check_elem_align(d_vectors, type));
+    if (row_stride < rows->dim && count > 1) return fail(CUDDLE_ERR_BAD_ARG, "row_stride %llu < dim %u", (unsigned long long)row_stride, rows->dim);
+    if (first_row > rows->n || count > rows->n - first_row) return fail(CUDDLE_ERR_BAD_ARG, "rows [%llu, +%llu) of %llu", (unsigned long long)first_row, (unsigned long long)count, (unsigned long long)rows->n);
+    DeviceGuard guard;
+    ST_TRY(guard.enter(device_id));
+    if (count == 0) return CUDDLE_OK;
+    const uint64_t tiles = (first_row % 16 + count + 15) / 16;
+    const bool vec = aligned16(d_vectors) && row_stride * type_size(type) % 16 == 0;
+    with_type(type, [&](auto z) {
+        using T = decltype(z);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(grid_for(tiles)), dim3(256), 0, (hipStream_t)stream_, (const T *)d_vectors, row_stride, first_row, count, rows->dim,
+                               rows->group, (uint8_t *)rows->codes, (uint16_t *)rows->scales, (double *)rows->sqnorm, tiles);
+        };
+        if (vec) go(int4_encode_kernel<T, true>);
+        else go(int4_encode_kernel<T, false>);
+    });
+    HIP_TRY(hipGetLastError());
+    return CUDDLE_OK;
+}
+
+extern "C" cuddle_status cuddle_int4_lookup_device(const cuddle_int4_rows *rows, const void *d_ids, uint32_t id_bits, uint64_t n_ids, float scale, uint32_t out_type,
+                                                   void *d_out, int device_id, void *stream_) {
+    ST_TRY(check_rows(rows, false));
+    ST_TRY(check_type(out_type));
+    ST_TRY(check_ids(d_ids, id_bits));
+    if (n_ids && !d_out) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    if (!d_ids && n_ids > rows->n) return fail(CUDDLE_ERR_BAD_ARG, "%llu rows of %llu", (unsigned long long)n_ids, (unsigned long long)rows->n);
+    ST_TRY(check_elem_align(d_out, out_type));
+    DeviceGuard guard;
+    ST_TRY(guard.enter(device_id));
+    if (n_ids == 0) return CUDDLE_OK;
+    const uint32_t ppr = (rows->dim + 7) / 8, rpb = std::max<uint32_t>(1, 256 / ppr);
+    const bool vec = aligned16(d_out) && (uint64_t)rows->dim * type_size(out_type) % 16 == 0;
+    with_type(out_type, [&](auto z) {
+        using T = decltype(z);
+        with_id(id_bits, [&](auto zi) {
+            using I = decltype(zi);
+            auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3(grid_for((n_ids + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream_, (const uint8_t *)rows->codes,
+                                   (const uint16_t *)rows->scales, rows->n, rows->dim, rows->group, (const I *)d_ids, n_ids, scale, (T *)d_out, rpb);
+            };
+            if (vec) go(int4_lookup_kernel<T, I, true>);
+            else go(int4_lookup_kernel<T, I, false>);
+        });
+    });
+    HIP_TRY(hipGetLastError());
+    return CUDDLE_OK;
+}
+
+extern "C" cuddle_status cuddle_int4_workspace(uint64_t n, uint32_t dim, uint32_t n_queries, uint32_t k, uint64_t *bytes) {
+    if (!bytes) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    ST_TRY(check_dim(dim));
+    if (n >= 0xFFFFFFFFull) return fail(CUDDLE_ERR_UNSUPPORTED, "%llu rows: fewer than 2^32 - 1", (unsigned long long)n);
+    if (k > kTopMaxK) return fail(CUDDLE_ERR_UNSUPPORTED, "k %u > %u", k, kTopMaxK);
+    *bytes = int4_ws(n, dim, n_queries, k).bytes;
+    return CUDDLE_OK;
+}
+
+extern "C" cuddle_status cuddle_int4_distances_device(const cuddle_int4_rows *rows, const void *d_queries, uint32_t type, uint32_t n_queries, uint32_t metric,
+                                                      float *d_dist, void *d_ws, uint64_t ws_bytes, int device_id, void *stream_) {
+    ST_TRY(check_query_call(rows, d_queries, type, n_queries, metric));
+    if (n_queries && rows->n && !d_dist) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    const Int4Ws w = int4_ws(rows->n, rows->dim, n_queries, 0);
+    if (n_queries && rows->n) ST_TRY(check_ws(d_ws, ws_bytes, w.bytes));
+    DeviceGuard guard;
+    ST_TRY(guard.enter(device_id));
+    if (n_queries == 0 || rows->n == 0) return CUDDLE_OK;
+    for (uint32_t q0 = 0; q0 < n_queries; q0 += w.qc)
+        ST_TRY(int4_distances_round(rows, d_queries, type, q0, std::min(w.qc, n_queries - q0), metric, d_dist + (uint64_t)q0 * rows->n, rows->n, (uint8_t *)d_ws, w,
+                                    (hipStream_t)stream_));
+    return CUDDLE_OK;
+}
+
+extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows, const void *d_queries, uint32_t type, uint32_t n_queries, uint32_t k,
+                                                   uint32_t metric, uint64_t *d_out_ids, float *d_out_dist, uint32_t *d_out_count, void *d_ws, uint64_t ws_bytes,
+                                                   int device_id, void *stream_) {
+    hipStream_t s = (hipStream_t)stream_;
+    ST_TRY(check_query_call(rows, d_queries, type, n_queries, metric));
+    if (k == 0) return fail(CUDDLE_ERR_BAD_ARG, "k must be >= 1");
+    if (k > kTopMaxK) return fail(CUDDLE_ERR_UNSUPPORTED, "k %u > %u", k, kTopMaxK);
+    if (n_queries && (!d_out_ids || !d_out_dist)) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    const Int4Ws w = int4_ws(rows->n, rows->dim, n_queries, k);
+    if (n_queries && rows->n) ST_TRY(check_ws(d_ws, ws_bytes, w.bytes));
+    DeviceGuard guard;
+    ST_TRY(guard.enter(device_id));
+    if (n_queries == 0) return CUDDLE_OK;
+    if (rows->n == 0) {
+        const uint64_t total = (uint64_t)n_queries * k;
+        hipLaunchKernelGGL(int4_topk_none_kernel, dim3(grid_for((total + 255) / 256)), dim3(256), 0, s, d_out_ids, d_out_dist, d_out_count, total, n_queries);
+        HIP_TRY(hipGetLastError());
+        return CUDDLE_OK;
+    }
+    uint8_t *ws = (uint8_t *)d_ws;
+    float *dist = (float *)(ws + w.dist);
+    const uint32_t found = (uint32_t)std::min<uint64_t>(k, rows->n);
+    for (uint32_t q0 = 0; q0 < n_queries; q0 += w.qc) {
+        const uint32_t nq = std::min(w.qc, n_queries - q0);
+        ST_TRY(int4_distances_round(rows, d_queries, type, q0, nq, metric, dist, rows->n, ws, w, s));
+        const void *in = dist;
+        uint64_t stride = rows->n, items = rows->n;
+        int level = 0;
+        for (; items > kTopChunk; ++level) {
+            const uint64_t parts = (items + kTopChunk - 1) / kTopChunk;
+            uint64_t *out = (uint64_t *)(ws + w.sel[level & 1]);
+            if (level == 0) hipLaunchKernelGGL(int4_topk_level_kernel<true>, dim3((unsigned)parts, nq), dim3(256), 0, s, in, stride, items, k, out);
+            else hipLaunchKernelGGL(int4_topk_level_kernel<false>, dim3((unsigned)parts, nq), dim3(256), 0, s, in, stride, items, k, out);
+            in = out;
+            stride = items = parts * k;
+        }
+        uint64_t *ids = d_out_ids + (uint64_t)q0 * k;
+        float *od = d_out_dist + (uint64_t)q0 * k;
+        uint32_t *oc = d_out_count ? d_out_count + q0 : nullptr;
+        if (level == 0) hipLaunchKernelGGL(int4_topk_final_kernel<true>, dim3(nq), dim3(256), 0, s, in, stride, (uint32_t)items, k, found, dist, rows->n, ids, od, oc);
+        else hipLaunchKernelGGL(int4_topk_final_kernel<false>, dim3(nq), dim3(256), 0, s, in, stride, (uint32_t)items, k, found, dist, rows->n, ids, od, oc);
+        HIP_TRY(hipGetLastError());
+    }
+    return CUDDLE_OK;
+}
+
+extern "C" cuddle_status cuddle_rows_lookup_device(const void *d_table, uint32_t type, uint64_t row_stride, uint64_t n_rows, uint32_t dim, const void *d_ids,
+                                                   uint32_t id_bits, uint64_t n_ids, float scale, void *d_out, int device_id, void *stream_) {
+    ST_TRY(check_type(type));
+    ST_TRY(check_dim(dim));
+    ST_TRY(check_ids(d_ids, id_bits));
+    if (n_ids && (!d_ids || !d_out || (n_rows && !d_table))) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    if (row_stride < dim && n_rows > 1) return fail(CUDDLE_ERR_BAD_ARG, "row_stride %llu < dim %u", (unsigned long long)row_stride, dim);
+    ST_TRY(check_elem_align(d_table, type));
+    ST_TRY(check_elem_align(d_out, type));
+    DeviceGuard guard;
+    ST_TRY(guard.enter(device_id));
+    if (n_ids == 0) return CUDDLE_OK;
+    const uint32_t ts = type_size(type);
+    const bool vec = aligned16(d_table) && aligned16(d_out) && row_stride * ts % 16 == 0 && (uint64_t)dim * ts % 16 == 0;
+    const uint32_t per = vec ? 16 / ts : 1, ppr = (dim + per - 1) / per, rpb = std::max<uint32_t>(1, 256 / ppr);
+    with_type(type, [&](auto z) {
+        using T = decltype(z);
+        with_id(id_bits, [&](auto zi) {
+            using I = decltype(zi);
+            auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3(grid_for((n_ids + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream_, (const T *)d_table, row_stride, n_rows, dim,
+                                   (const I *)d_ids, n_ids, scale, (T *)d_out, rpb);
+            };
+            if (vec) go(rows_lookup_kernel<T, I, 16 / sizeof(T)>);
+            else go(rows_lookup_kernel<T, I, 1>);
+        });
+    });
+    HIP_TRY(hipGetLastError());
+    return CUDDLE_OK;
+}
+
+namespace {
+struct GradWs {
+    size_t key[2], pos[2], hist, bytes;
+};
+GradWs grad_ws(uint64_t n_ids) {
+    GradWs w{};
+    size_t at = 0;
+    for (int i = 0; i < 2; ++i) {
+        w.key[i] = at;
+        at += round_ws(n_ids * 4);
+        w.pos[i] = at;
+        at += round_ws(n_ids * 4);
+    }
+    w.hist = at;
+    at += round_ws((n_ids + kSortTile - 1) / kSortTile * 1024);
+    w.bytes = at;
+    return w;
+}
+cuddle_status check_grad_sizes(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
+    ST_TRY(check_dim(dim));
+    if (n_rows >= 0xFFFFFFFFull) return fail(CUDDLE_ERR_UNSUPPORTED, "%llu rows: fewer than 2^32 - 1", (unsigned long long)n_rows);
+    if (n_ids >= (1ull << 31)) return fail(CUDDLE_ERR_UNSUPPORTED, "%llu ids: fewer than 2^31", (unsigned long long)n_ids);
+    return CUDDLE_OK;
+}
+} // namespace
+
+extern "C" cuddle_status cuddle_rows_grad_workspace(uint64_t n_ids, uint64_t n_rows, uint32_t dim, uint64_t *bytes) {
+    if (!bytes) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    ST_TRY(check_grad_sizes(n_ids, n_rows, dim));
+    *bytes = grad_ws(n_ids).bytes;
+    return CUDDLE_OK;
+}
+
+extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_t type, uint64_t row_stride, const void *d_ids, uint32_t id_bits, uint64_t n_ids,
+                                                 float scale, uint64_t n_rows, uint32_t dim, uint32_t flags, uint32_t grad_type, void *d_grad, void *d_ws,
+                                                 uint64_t ws_bytes, int device_id, void *stream_) {
+    hipStream_t s = (hipStream_t)stream_;
+    ST_TRY(check_type(type));
+    ST_TRY(check_type(grad_type));
+    ST_TRY(check_grad_sizes(n_ids, n_rows, dim));
+    ST_TRY(check_ids(d_ids, id_bits));
+    if (flags & ~CUDDLE_GRAD_ACCUMULATE) return fail(CUDDLE_ERR_BAD_ARG, "unknown flags 0x%x", flags);
+    if ((n_ids && (!d_grad_out || !d_ids)) || (n_rows && !d_grad)) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
+    if (row_stride < dim && n_ids > 1) return fail(CUDDLE_ERR_BAD_ARG, "row_stride %llu < dim %u", (unsigned long long)row_stride, dim);
+    ST_TRY(check_elem_align(d_grad_out, type));
+    ST_TRY(check_elem_align(d_grad, grad_type));
+    const GradWs w = grad_ws(n_ids);
+    if (n_ids && n_rows) ST_TRY(check_ws(d_ws, ws_bytes, w.bytes));
+    DeviceGuard guard;
+    ST_TRY(guard.enter(device_id));
+    if (n_rows == 0) return CUDDLE_OK;
+    const bool add = flags & CUDDLE_GRAD_ACCUMULATE;
+    if (!add)
+        with_type(grad_type, [&](auto z) {
+            using O = decltype(z);
+            const uint64_t total = n_rows * dim;
+            hipLaunchKernelGGL(rows_zero_kernel<O>, dim3(grid_for((total + 255) / 256)), dim3(256), 0, s, (O *)d_grad, total);
+        });
+    if (n_ids == 0) {
+        HIP_TRY(hipGetLastError());
+        return CUDDLE_OK;
+    }
+    uint8_t *ws = (uint8_t *)d_ws;
+    uint32_t *key[2] = {(uint32_t *)(ws + w.key[0]), (uint32_t *)(ws + w.key[1])}, *pos[2] = {(uint32_t *)(ws + w.pos[0]), (uint32_t *)(ws + w.pos[1])};
+    uint32_t *hist = (uint32_t *)(ws + w.hist);
+    const uint32_t t = (uint32_t)n_ids, tiles = (t + kSortTile - 1) / kSortTile;
+    with_id(id_bits, [&](auto zi) {
+        using I = decltype(zi);
+        hipLaunchKernelGGL(rows_key_kernel<I>, dim3(grid_for((n_ids + 255) / 256)), dim3(256), 0, s, (const I *)d_ids, n_ids, n_rows, key[0], pos[0]);
+    });
+    int cur = 0;
+    for (uint32_t shift = 0; shift < 32 && (n_rows >> shift); shift += 8, cur ^= 1) {
+        hipLaunchKernelGGL(rows_sort_hist_kernel, dim3(tiles), dim3(256), 0, s, key[cur], t, shift, hist);
+        hipLaunchKernelGGL(rows_sort_scan_kernel, dim3(1), dim3(256), 0, s, hist, tiles);
+        hipLaunchKernelGGL(rows_sort_scatter_kernel, dim3(tiles), dim3(256), 0, s, key[cur], pos[cur], t, shift, hist, key[cur ^ 1], pos[cur ^ 1]);
+    }
+    with_type(type, [&](auto z) {
+        using T = decltype(z);
+        with_type(grad_type, [&](auto zo) {
+            using O = decltype(zo);
+            hipLaunchKernelGGL((rows_grad_kernel<T, O>), dim3(grid_for((n_ids + 3) / 4)), dim3(256), 0, s, (const T *)d_grad_out, row_stride, key[cur], pos[cur], t,
+                               n_rows, dim, scale, add ? 1u : 0u, (O *)d_grad);
+        });
+    });
+    HIP_TRY(hipGetLastError());
+    return CUDDLE_OK;
+}

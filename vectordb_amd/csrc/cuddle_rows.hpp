@@ -1,0 +1,623 @@
+// cuddle_rows.hpp — an embedding table on the device: 4-bit rows with group scales (encoding, decoding, distances of
+// a few queries to every row, exhaustive top-k), row lookup by id, and the gradient of that lookup.
+// No counterpart in the reference, whose codes are 1-bit (src/quantization/binary.rs, rabitq.rs) and whose rows are
+// fetched one at a time (MmapVectorStore::get, src/storage/mmap.rs:106-115).
+//
+// 4-bit rows. A row's components are cut into groups of G (32, 64 or 128); group g has the scale
+//   s = bf16(max|x| / 7)   and the codes   c = rint(x / s) (halves to even, clamped to -7..7),   and stands for s * c.
+// A group whose scale rounds to zero has codes 0; a group that holds a NaN or an infinity gets s = NaN and codes 0,
+// so it decodes to NaN and every distance of the row is NaN.
+//
+// Layout. What a wave wants to load is what one matrix instruction eats: 16 rows x 64 components of int8, lane
+// (r = lane & 15, h = lane >> 4) holding 16 components of row r. So codes are stored in units of 16 rows x 64
+// components (512 bytes, rows of 32 bytes), units of a tile of 16 rows one after the other:
+//   byte h * 8 + i of a row's unit = component 8h + i in the low nibble, 32 + 8h + i in the high nibble (i < 8),
+// two's complement. A wave reads 8 bytes per lane, 512 contiguous bytes, and has both halves of the operand after a
+// shift and two masks; the code stays in the high nibble of its byte, so the products come out 16 times too large
+// (an exact factor, taken out at the end). Scales are row-major: [rows][gstride] bf16, gstride even.
+#pragma once
+
+#include "cuddle_kernels.hpp"
+
+namespace cuddle {
+
+typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2;
+constexpr uint32_t kInt4Unit = 64;      // components per unit
+constexpr uint32_t kInt4UnitBytes = 512; // 16 rows x 32 bytes
+
+__host__ __device__ __forceinline__ uint32_t int4_units(uint32_t dim) { return (dim + kInt4Unit - 1) / kInt4Unit; }
+__host__ __device__ __forceinline__ uint32_t int4_gstride(uint32_t dim, uint32_t group) {
+    return ((dim + group - 1) / group + 1) & ~1u;
+}
+
+// ---- element types ---------------------------------------------------------------------------
+struct Bf16 { uint16_t b; };
+__device__ __forceinline__ float bf16_to_f32(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+__device__ __forceinline__ uint16_t f32_to_bf16(float f) { // to nearest, halves to even; NaN stays NaN
+    const uint32_t u = __float_as_uint(f);
+    if (f != f) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(Bf16 v) { return bf16_to_f32(v.b); }
+template <class T> __device__ __forceinline__ T from_f32(float f);
+template <> __device__ __forceinline__ float from_f32<float>(float f) { return f; }
+// The value as it stands, then rounded: without the barrier the compiler folds a product before it and this rounding
+// into one mixed-precision instruction, whose single rounding is not the product's f32 rounding followed by this one.
+template <> __device__ __forceinline__ _Float16 from_f32<_Float16>(float f) {
+    asm("" : "+v"(f));
+    return (_Float16)f;
+}
+template <> __device__ __forceinline__ Bf16 from_f32<Bf16>(float f) { return Bf16{f32_to_bf16(f)}; }
+
+// N consecutive elements moved as one piece (the caller has checked the alignment).
+template <class T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+
+// Eight consecutive components of a row as f32, zeros from `dim` on.
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T *row, uint32_t e0, uint32_t dim, float (&x)[8]) {
+    if (VEC && e0 + 8 <= dim) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int p = 0; p < 8 / N; ++p) {
+            const Pack<T, N> v = *reinterpret_cast<const Pack<T, N> *>(row + e0 + p * N);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[p * N + i] = to_f32(v.v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = e0 + i < dim ? to_f32(row[e0 + i]) : 0.f;
+    }
+}
+
+// Eight components to a row of outputs, those below `dim`.
+template <class T, bool VEC>
+__device__ __forceinline__ void store8(T *row, uint32_t e0, uint32_t dim, const float (&x)[8]) {
+    if (VEC && e0 + 8 <= dim) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int p = 0; p < 8 / N; ++p) {
+            Pack<T, N> v;
+#pragma unroll
+            for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(x[p * N + i]);
+            *reinterpret_cast<Pack<T, N> *>(row + e0 + p * N) = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (e0 + i < dim) row[e0 + i] = from_f32<T>(x[i]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// encoding
+// ---------------------------------------------------------------------------------------------
+// The code of x under scale s > 0 (inv = 1 / s, or 0 where that overflows): rint(x / s), exactly. s has 8 significant
+// bits and |n| <= 8, so n * s is exact; x - n * s is a multiple of the last place of x and no larger than x (or s),
+// so the fma returns it exactly and comparing it with s / 2 decides the rounding, whatever the estimate n was off by.
+__device__ __forceinline__ int32_t int4_code(float x, float s, float inv) {
+    float n = rintf(inv != 0.f ? x * inv : x / s);
+    n = fminf(fmaxf(n, -8.f), 8.f);
+    const float r = __builtin_fmaf(-n, s, x), h = 0.5f * s;
+    if (fabsf(r) > h || (fabsf(r) == h && ((int32_t)n & 1))) n += r > 0.f ? 1.f : -1.f;
+    return (int32_t)fminf(fmaxf(n, -7.f), 7.f);
+}
+
+// One block = one tile of 16 rows, 16 lanes per row; a lane has 8 consecutive components, the 16 lanes of a row two
+// units (128 components) per step. The group's largest magnitude is a reduction over G / 8 neighbouring lanes; the low
+// and the high nibbles of a byte come from lanes 4 apart. Rows outside [first, first + count) are left alone.
+// sqnorm[r] = sum over groups of s^2 * sum c^2 in f64 (the integer sums are exact).
+// Bound by the read of the rows. grid = tiles touched (x stride), block 256.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256)
+int4_encode_kernel(const T *x, uint64_t stride, uint64_t first, uint64_t count, uint32_t dim, uint32_t group, uint8_t *codes,
+                   uint16_t *scales, double *sqnorm, uint64_t tiles) {
+    const uint32_t units = int4_units(dim), gs = int4_gstride(dim, group), lane16 = threadIdx.x & 15, r = threadIdx.x >> 4;
+    const uint32_t jj = lane16 & 7;
+    for (uint64_t t = first / 16 + blockIdx.x; t < first / 16 + tiles; t += gridDim.x) {
+        const uint64_t row = t * 16 + r;
+        const bool act = row >= first && row < first + count;
+        const T *src = x + (act ? row - first : 0) * stride;
+        double sq = 0.0;
+        for (uint32_t u0 = 0; u0 < units; u0 += 2) {
+            const uint32_t u = u0 + (lane16 >> 3), e0 = u * kInt4Unit + jj * 8;
+            float v[8];
+            if (act)
+                load8<T, VEC>(src, e0, dim, v);
+            else
+                for (int i = 0; i < 8; ++i) v[i] = 0.f;
+            float a = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float m = fabsf(v[i]);
+                a = fmaxf(a, m <= 3.4028234663852886e38f ? m : __builtin_huge_valf()); // NaN counts as infinite
+            }
+            a = fmaxf(a, __shfl_xor(a, 1, 64));
+            a = fmaxf(a, __shfl_xor(a, 2, 64));
+            if (group >= 64) a = fmaxf(a, __shfl_xor(a, 4, 64));
+            if (group >= 128) a = fmaxf(a, __shfl_xor(a, 8, 64));
+            const bool bad = a > 3.4028234663852886e38f;
+            const uint16_t sb = bad ? (uint16_t)0x7FC0u : f32_to_bf16(a / 7.0f);
+            const float s = bf16_to_f32(sb);
+            const float inv = s >= 1e-30f ? 1.0f / s : 0.f;
+            int32_t c[8], c2 = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = (bad || s == 0.f) ? 0 : int4_code(v[i], s, inv);
+                c2 += c[i] * c[i];
+            }
+            sq = __builtin_fma((double)s * (double)s, (double)c2, sq);
+            uint32_t p0 = 0, p1 = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p0 |= ((uint32_t)c[i] & 15u) << (8 * i);
+                p1 |= ((uint32_t)c[i + 4] & 15u) << (8 * i);
+            }
+            const uint32_t q0 = (uint32_t)__shfl_xor((int)p0, 4, 64), q1 = (uint32_t)__shfl_xor((int)p1, 4, 64);
+            if (act && u < units) {
+                if (jj < 4)
+                    *reinterpret_cast<uint2 *>(codes + (t * units + u) * kInt4UnitBytes + r * 32 + jj * 8) = make_uint2(p0 | q0 << 4, p1 | q1 << 4);
+                const uint32_t g = e0 / group;
+                if (e0 % group == 0 && g < gs) scales[row * gs + g] = sb;
+            }
+        }
+        // a padding group of the scales' row that no lane above stands for
+        if (act && lane16 == 0 && (uint64_t)(gs - 1) * group >= (uint64_t)units * kInt4Unit) scales[row * gs + gs - 1] = 0;
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) sq += __shfl_xor(sq, m, 64);
+        if (act && lane16 == 0) sqnorm[row] = sq;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// lookup
+// ---------------------------------------------------------------------------------------------
+// ids: 32- or 64-bit, signed; anything outside [0, n) gives `none`.
+constexpr uint64_t kNoRow = ~0ull;
+template <class I>
+__device__ __forceinline__ uint64_t row_of_id(const I *ids, uint64_t t, uint64_t n) {
+    const int64_t i = (int64_t)ids[t];
+    return i >= 0 && (uint64_t)i < n ? (uint64_t)i : kNoRow;
+}
+
+// out[t] = scale * table[ids[t]]; a block takes `rpb` outputs at a time and its threads the pieces of their rows, N
+// elements each. Bound by the writes (and the reads where the rows are not found in a cache).
+template <class T, class I, int N>
+__global__ void __launch_bounds__(256)
+rows_lookup_kernel(const T *table, uint64_t stride, uint64_t n, uint32_t dim, const I *ids, uint64_t n_ids, float scale, T *out, uint32_t rpb) {
+    const uint32_t ppr = (dim + N - 1) / N;
+    for (uint64_t t0 = (uint64_t)blockIdx.x * rpb; t0 < n_ids; t0 += (uint64_t)gridDim.x * rpb) {
+        const uint32_t items = (uint32_t)min((uint64_t)rpb, n_ids - t0) * ppr;
+        for (uint32_t it = threadIdx.x; it < items; it += 256) {
+            const uint32_t rr = it / ppr, p = it - rr * ppr;
+            const uint64_t t = t0 + rr, row = row_of_id(ids, t, n);
+            Pack<T, N> v;
+            if (row != kNoRow) {
+                v = *reinterpret_cast<const Pack<T, N> *>(table + row * stride + (uint64_t)p * N);
+#pragma unroll
+                for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(to_f32(v.v[i]) * scale);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(0.f);
+            }
+            *reinterpret_cast<Pack<T, N> *>(out + t * dim + (uint64_t)p * N) = v;
+        }
+    }
+}
+
+// The same from 4-bit rows: a piece is 8 components, one nibble of each of 8 bytes (lanes 4 apart share the bytes).
+// s * c has 12 significant bits, so only the product with `scale` and the rounding to the output's type round.
+// ids == nullptr: rows 0 .. n_ids - 1 in order.
+template <class T, class I, bool VEC>
+__global__ void __launch_bounds__(256)
+int4_lookup_kernel(const uint8_t *codes, const uint16_t *scales, uint64_t n, uint32_t dim, uint32_t group, const I *ids, uint64_t n_ids, float scale,
+                   T *out, uint32_t rpb) {
+    const uint32_t units = int4_units(dim), gs = int4_gstride(dim, group), ppr = (dim + 7) / 8;
+    for (uint64_t t0 = (uint64_t)blockIdx.x * rpb; t0 < n_ids; t0 += (uint64_t)gridDim.x * rpb) {
+        const uint32_t items = (uint32_t)min((uint64_t)rpb, n_ids - t0) * ppr;
+        for (uint32_t it = threadIdx.x; it < items; it += 256) {
+            const uint32_t rr = it / ppr, p = it - rr * ppr;
+            const uint64_t t = t0 + rr, row = ids ? row_of_id(ids, t, n) : t;
+            float x[8];
+            if (row != kNoRow) {
+                const uint32_t u = p >> 3, jj = p & 7;
+                uint2 w = *reinterpret_cast<const uint2 *>(codes + ((row >> 4) * units + u) * kInt4UnitBytes + (uint32_t)(row & 15) * 32 + (jj & 3) * 8);
+                if (jj < 4) {
+                    w.x <<= 4;
+                    w.y <<= 4;
+                }
+                const float s = bf16_to_f32(scales[row * gs + p * 8 / group]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = s * (float)((int32_t)(w.x << (24 - 8 * i)) >> 28) * scale;
+                    x[i + 4] = s * (float)((int32_t)(w.y << (24 - 8 * i)) >> 28) * scale;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = 0.f;
+            }
+            store8<T, VEC>(out + t * dim, p * 8, dim, x);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// distances of queries to 4-bit rows
+// ---------------------------------------------------------------------------------------------
+// The query side of the products. A query is written in fixed point, q_i = Q_i * 2^(e - 30) with |Q_i| <= 2^30, e from
+// its largest magnitude, and Q_i as four signed base-256 digits: with the codes as they are, every product and every
+// sum over a group is then an exact integer product of int8 on the matrix cores. What is rounded is q_i itself, by at
+// most 2^-31 of the largest |q| - f16 and bf16 queries, and whole numbers, not at all in practice.
+// Operand order: [query quartet][unit][lane][16 bytes], lane = (h << 4) | (query & 3) << 2 | digit, byte b = component
+// 8h + b (b < 8) or 32 + 8h + b - 8 of the unit.
+struct Int4Query {
+    double scale; // value of one unit of the products' last place, 2^(e - 34); NaN for a query with a non-finite value
+    double sq;    // |q|^2
+};
+
+template <class T>
+__global__ void __launch_bounds__(256)
+int4_query_kernel(const T *queries, uint32_t nq, uint32_t dim, uint32_t units, uint8_t *dig, Int4Query *info) {
+    __shared__ float s_max[4];
+    __shared__ double s_sq[4];
+    const uint32_t q = blockIdx.x, tid = threadIdx.x;
+    const bool real = q < nq; // the last quartet is filled up with zero queries
+    const T *src = queries + (uint64_t)(real ? q : 0) * dim;
+    float m = 0.f;
+    double sq = 0.0;
+    if (real)
+        for (uint32_t i = tid; i < dim; i += 256) {
+            const float v = to_f32(src[i]), a = fabsf(v);
+            m = fmaxf(m, a <= 3.4028234663852886e38f ? a : __builtin_huge_valf());
+            sq = __builtin_fma((double)v, (double)v, sq);
+        }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        m = fmaxf(m, __shfl_xor(m, d, 64));
+        sq += __shfl_xor(sq, d, 64);
+    }
+    if ((tid & 63) == 0) {
+        s_max[tid >> 6] = m;
+        s_sq[tid >> 6] = sq;
+    }
+    __syncthreads();
+    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const bool bad = m > 3.4028234663852886e38f;
+    int e = 0;
+    if (!bad && m > 0.f) (void)frexp((double)m, &e);
+    const double up = ldexp(1.0, 30 - e);
+    if (tid == 0 && real) info[q] = Int4Query{bad ? __builtin_nan("") : ldexp(1.0, e - 34), (s_sq[0] + s_sq[1]) + (s_sq[2] + s_sq[3])};
+    uint8_t *dst = dig + (uint64_t)(q >> 2) * units * 1024;
+    for (uint32_t i = tid; i < units * kInt4Unit; i += 256) {
+        const float v = real && i < dim && !bad ? to_f32(src[i]) : 0.f;
+        int32_t f = (int32_t)rint((double)v * up);
+        const uint32_t u = i >> 6, e6 = i & 63, h = (e6 & 31) >> 3, b = ((e6 >> 5) << 3) | (e6 & 7);
+#pragma unroll
+        for (uint32_t d = 0; d < 4; ++d) {
+            const int32_t lo = (int32_t)(int8_t)(f & 255);
+            f = (f - lo) >> 8;
+            dst[(uint64_t)u * 1024 + ((h << 4) | ((q & 3) << 2) | d) * 16 + b] = (uint8_t)lo;
+        }
+    }
+}
+
+// One group's integer products into the running sum: c = the four digits' products of (row r, query h).
+__device__ __forceinline__ double int4_group_sum(double acc, i32x4_t c, double s) {
+    const int32_t lo = c[0] + (c[1] << 8), hi = c[2] + (c[3] << 8);
+    return __builtin_fma(s, __builtin_fma((double)hi, 65536.0, (double)lo), acc);
+}
+
+// distance from the product: l2 |x|^2 + |q|^2 - 2p, cosine 1 - p / (|x||q|), dot -p; in f64, rounded once.
+__device__ __forceinline__ float int4_finish(uint32_t metric, double p, double xsq, double qsq) {
+    double d;
+    if (metric == kMetricDot)
+        d = -p;
+    else if (metric == kMetricCosine)
+        d = 1.0 - p / (sqrt(xsq) * sqrt(qsq));
+    else {
+        d = (xsq + qsq) - 2.0 * p;
+        d = d < 0.0 ? 0.0 : d; // the three terms of a row next to the query round apart
+    }
+    return (float)d;
+}
+
+// One wave: T tiles of 16 rows against QT quartets of queries. Weights are the B operand (a lane has one row), digits the
+// A operand, so that a lane receives the four digits of one (row, query) pair and puts them together itself: per group
+// and pair two integer adds and four f64 operations (f64 runs at the rate of f32 here).
+template <int G, int QT, int T>
+__global__ void __launch_bounds__(256)
+int4_distance_kernel(const uint8_t *codes, const uint16_t *scales, const double *sqnorm, uint64_t n, uint32_t dim, const uint8_t *dig,
+                     const Int4Query *info, uint32_t nq, uint32_t metric, float *dist, uint64_t dstride) {
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
+    const uint32_t units = int4_units(dim), gs = int4_gstride(dim, G);
+    const uint64_t tiles = (n + 15) / 16, groups = (tiles + T - 1) / T;
+    const uint8_t *dg = dig + (uint64_t)blockIdx.y * QT * units * 1024 + lane * 16;
+    for (uint64_t tg = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); tg < groups; tg += (uint64_t)gridDim.x * 4) {
+        const uint8_t *wp[T];
+        const uint16_t *sp[T];
+        double acc[T][QT];
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const uint64_t tile = min(tg * T + t, tiles - 1);
+            wp[t] = codes + tile * units * kInt4UnitBytes + r * 32 + h * 8;
+            sp[t] = scales + min(tile * 16 + r, n - 1) * gs;
+#pragma unroll
+            for (int q = 0; q < QT; ++q) acc[t][q] = 0.0;
+        }
+        i32x4_t c[T][QT];
+        for (uint32_t u = 0; u < units; ++u) {
+            i32x4_t a[QT];
+#pragma unroll
+            for (int q = 0; q < QT; ++q) a[q] = *reinterpret_cast<const i32x4_t *>(dg + ((uint64_t)q * units + u) * 1024);
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(wp[t] + (uint64_t)u * kInt4UnitBytes);
+                constexpr uint32_t M = 0xF0F0F0F0u;
+                const i32x4_t b = {(int)((w.x << 4) & M), (int)((w.y << 4) & M), (int)(w.x & M), (int)(w.y & M)};
+                const i32x4_t zero = {0, 0, 0, 0};
+                if (G == 32) {
+                    const double s0 = (double)bf16_to_f32(sp[t][2 * u]);
+                    const double s1 = (double)bf16_to_f32(sp[t][2 * u + 1]);
+                    const long b0 = (long)(uint32_t)b[0] | (long)((uint64_t)(uint32_t)b[1] << 32), b1 = (long)(uint32_t)b[2] | (long)((uint64_t)(uint32_t)b[3] << 32);
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) {
+                        const long a0 = (long)(uint32_t)a[q][0] | (long)((uint64_t)(uint32_t)a[q][1] << 32), a1 = (long)(uint32_t)a[q][2] | (long)((uint64_t)(uint32_t)a[q][3] << 32);
+                        acc[t][q] = int4_group_sum(acc[t][q], __builtin_amdgcn_mfma_i32_16x16x32_i8(a0, b0, zero, 0, 0, 0), s0);
+                        acc[t][q] = int4_group_sum(acc[t][q], __builtin_amdgcn_mfma_i32_16x16x32_i8(a1, b1, zero, 0, 0, 0), s1);
+                    }
+                } else if (G == 64) {
+                    const double s = (double)bf16_to_f32(sp[t][u]);
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) acc[t][q] = int4_group_sum(acc[t][q], __builtin_amdgcn_mfma_i32_16x16x64_i8(a[q], b, zero, 0, 0, 0), s);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) c[t][q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[q], b, u & 1 ? c[t][q] : zero, 0, 0, 0);
+                    if ((u & 1) || u + 1 == units) {
+                        const double s = (double)bf16_to_f32(sp[t][u >> 1]);
+#pragma unroll
+                        for (int q = 0; q < QT; ++q) acc[t][q] = int4_group_sum(acc[t][q], c[t][q], s);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const uint64_t row = (tg * T + t) * 16 + r;
+            if (row >= n) continue;
+            const double xsq = metric == kMetricDot ? 0.0 : sqnorm[row];
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+                const uint32_t qi = (blockIdx.y * QT + q) * 4 + h;
+                if (qi < nq) dist[qi * dstride + row] = int4_finish(metric, acc[t][q] * info[qi].scale, xsq, info[qi].sq);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// top-k of rows of distances
+// ---------------------------------------------------------------------------------------------
+// A selection is a list of (key << 32 | row) in row order; keys are f32_key (NaN after everything). A level cuts a
+// query's items into chunks and keeps each chunk's k smallest keys, equal keys by position; chunks are in row order and
+// only the last can be short of k, so positions stay the order of the rows and the padding (~0) stays at the end.
+constexpr uint32_t kTopChunk = 8192;
+constexpr uint32_t kTopMaxK = 1024;
+
+// The k-th smallest (k >= 1) of the C >= k keys in LDS, by 8 bits at a time, and how many items with that key belong
+// to the k smallest. hist: 256 words + 2 of LDS. All threads of the block.
+__device__ __forceinline__ void block_kth_key(const uint32_t *keys, uint32_t C, uint32_t k, uint32_t *hist, uint32_t &T, uint32_t &budget) {
+    uint32_t prefix = 0, mask = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (uint32_t i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < C; i += blockDim.x)
+            if ((keys[i] & mask) == prefix) atomicAdd(&hist[(keys[i] >> shift) & 255], 1u);
+        __syncthreads();
+        if (threadIdx.x < 64) { // four bins per lane: the bin in which the running count reaches k
+            const uint32_t b = threadIdx.x * 4;
+            const uint32_t c0 = hist[b], c1 = hist[b + 1], c2 = hist[b + 2], c3 = hist[b + 3];
+            const uint32_t incl = wave_inclusive_sum(c0 + c1 + c2 + c3);
+            uint32_t run = incl - (c0 + c1 + c2 + c3);
+            if (run < k && k <= incl) {
+                uint32_t bin = b;
+                if (run + c0 < k) { run += c0; ++bin;
+                    if (run + c1 < k) { run += c1; ++bin;
+                        if (run + c2 < k) { run += c2; ++bin; } } }
+                hist[256] = bin;
+                hist[257] = k - run;
+            }
+        }
+        __syncthreads();
+        prefix |= hist[256] << shift;
+        mask |= 255u << shift;
+        k = hist[257];
+        __syncthreads();
+    }
+    T = prefix;
+    budget = k;
+}
+
+// Level: from f32 distances (FIRST) or from the previous level's lists. in: [nq][in_stride]; out: [nq][parts][k].
+// grid (parts, nq), block 256, LDS kTopChunk words.
+template <bool FIRST>
+__global__ void __launch_bounds__(256)
+int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint32_t k, uint64_t *out) {
+    __shared__ uint32_t keys[kTopChunk];
+    __shared__ uint32_t hist[258];
+    __shared__ uint32_t wtmp[8];
+    const uint64_t base = (uint64_t)blockIdx.x * kTopChunk;
+    const uint32_t C = (uint32_t)min((uint64_t)kTopChunk, items - base), tid = threadIdx.x;
+    const float *df = static_cast<const float *>(in) + (uint64_t)blockIdx.y * in_stride + base;
+    const uint64_t *dl = static_cast<const uint64_t *>(in) + (uint64_t)blockIdx.y * in_stride + base;
+    for (uint32_t i = tid; i < C; i += 256) keys[i] = FIRST ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
+    __syncthreads();
+    uint64_t *o = out + ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * k;
+    uint32_t T = 0xFFFFFFFFu, budget = C;
+    if (C > k) block_kth_key(keys, C, k, hist, T, budget);
+    ordered_threshold_compact(
+        C, T, budget, [&](uint32_t i) -> uint32_t { return keys[i]; },
+        [&](uint32_t i, uint32_t kv, uint32_t rank) { o[rank] = FIRST ? ((uint64_t)kv << 32 | (uint32_t)(base + i)) : dl[i]; }, wtmp);
+    for (uint32_t i = C + tid; i < k; i += 256) o[i] = ~0ull;
+}
+
+// Last level: at most kTopChunk items; the k smallest, in order, as ids and distances.
+template <bool FIRST>
+__global__ void __launch_bounds__(256)
+int4_topk_final_kernel(const void *in, uint64_t in_stride, uint32_t items, uint32_t k, uint32_t found, const float *dist, uint64_t dstride, uint64_t *ids,
+                       float *out, uint32_t *count) {
+    __shared__ uint32_t keys[kTopChunk];
+    __shared__ uint64_t sel[kTopMaxK];
+    __shared__ uint32_t hist[258];
+    __shared__ uint32_t wtmp[8];
+    const uint32_t tid = threadIdx.x, q = blockIdx.x;
+    const float *df = static_cast<const float *>(in) + (uint64_t)q * in_stride;
+    const uint64_t *dl = static_cast<const uint64_t *>(in) + (uint64_t)q * in_stride;
+    for (uint32_t i = tid; i < items; i += 256) keys[i] = FIRST ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
+    const uint32_t width = next_pow2(min(k, items));
+    for (uint32_t i = tid; i < width; i += 256) sel[i] = ~0ull;
+    __syncthreads();
+    uint32_t T = 0xFFFFFFFFu, budget = items;
+    if (items > k) block_kth_key(keys, items, k, hist, T, budget);
+    ordered_threshold_compact(
+        items, T, budget, [&](uint32_t i) -> uint32_t { return keys[i]; },
+        [&](uint32_t i, uint32_t kv, uint32_t rank) { sel[rank] = FIRST ? ((uint64_t)kv << 32 | i) : dl[i]; }, wtmp);
+    __syncthreads();
+    block_sort_u64(sel, width);
+    for (uint32_t i = tid; i < k; i += 256) {
+        const bool have = i < found;
+        const uint32_t row = have ? (uint32_t)sel[i] : 0u;
+        ids[(uint64_t)q * k + i] = have ? (uint64_t)row : ~0ull;
+        out[(uint64_t)q * k + i] = have ? dist[(uint64_t)q * dstride + row] : __builtin_huge_valf();
+    }
+    if (count && tid == 0) count[q] = found;
+}
+
+// An empty table's answer.
+__global__ void __launch_bounds__(256)
+int4_topk_none_kernel(uint64_t *ids, float *out, uint32_t *count, uint64_t total, uint32_t nq) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+        ids[i] = ~0ull;
+        out[i] = __builtin_huge_valf();
+        if (count && i < nq) count[i] = 0;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// gradient of the lookup
+// ---------------------------------------------------------------------------------------------
+// Stable radix sort of (row, position) by row, 8 bits per pass: tile histograms, their prefix sums, scatter. Ids
+// outside the table get the key n_rows and end up behind everything.
+constexpr uint32_t kSortTile = 2048;
+
+template <class I>
+__global__ void __launch_bounds__(256)
+rows_key_kernel(const I *ids, uint64_t t, uint64_t n_rows, uint32_t *key, uint32_t *pos) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < t; i += (uint64_t)gridDim.x * 256) {
+        const uint64_t r = row_of_id(ids, i, n_rows);
+        key[i] = r == kNoRow ? (uint32_t)n_rows : (uint32_t)r;
+        pos[i] = (uint32_t)i;
+    }
+}
+
+__global__ void __launch_bounds__(256)
+rows_sort_hist_kernel(const uint32_t *key, uint32_t t, uint32_t shift, uint32_t *hist) {
+    __shared__ uint32_t h[256];
+    h[threadIdx.x] = 0;
+    __syncthreads();
+    const uint32_t b = blockIdx.x * kSortTile, e = min(b + kSortTile, t);
+    for (uint32_t i = b + threadIdx.x; i < e; i += 256) atomicAdd(&h[(key[i] >> shift) & 255], 1u);
+    __syncthreads();
+    hist[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
+}
+
+// hist[tile][digit] -> where the tile's first key of that digit goes. One block of 256 threads, one per digit.
+__global__ void __launch_bounds__(256)
+rows_sort_scan_kernel(uint32_t *hist, uint32_t tiles) {
+    __shared__ uint32_t tot[257];
+    const uint32_t d = threadIdx.x;
+    uint32_t run = 0;
+    for (uint32_t i = 0; i < tiles; ++i) run += hist[i * 256 + d];
+    tot[d] = run;
+    __syncthreads();
+    wave0_exclusive_scan_lds(tot, 256);
+    __syncthreads();
+    run = tot[d];
+    for (uint32_t i = 0; i < tiles; ++i) {
+        const uint32_t v = hist[i * 256 + d];
+        hist[i * 256 + d] = run;
+        run += v;
+    }
+}
+
+// Each wave ranks its own 512 consecutive keys, 64 at a time: lanes with the same digit find each other by eight ballots.
+__global__ void __launch_bounds__(256)
+rows_sort_scatter_kernel(const uint32_t *key, const uint32_t *pos, uint32_t t, uint32_t shift, const uint32_t *hist, uint32_t *okey, uint32_t *opos) {
+    __shared__ uint32_t off[4][256];
+    const uint32_t tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    for (int v = 0; v < 4; ++v) off[v][tid] = 0;
+    __syncthreads();
+    const uint32_t b = blockIdx.x * kSortTile + w * (kSortTile / 4);
+    for (uint32_t i = 0; i < kSortTile / 4; i += 64)
+        if (b + i + lane < t) atomicAdd(&off[w][(key[b + i + lane] >> shift) & 255], 1u);
+    __syncthreads();
+    uint32_t run = hist[blockIdx.x * 256 + tid];
+    for (int v = 0; v < 4; ++v) {
+        const uint32_t c = off[v][tid];
+        off[v][tid] = run;
+        run += c;
+    }
+    __syncthreads();
+    for (uint32_t i = 0; i < kSortTile / 4; i += 64) {
+        const bool in = b + i + lane < t;
+        const uint32_t k = in ? key[b + i + lane] : 0u, d = (k >> shift) & 255;
+        uint64_t same = __ballot(in);
+#pragma unroll
+        for (int bit = 0; bit < 8; ++bit) {
+            const uint64_t m = __ballot((d >> bit) & 1);
+            same &= (d >> bit) & 1 ? m : ~m;
+        }
+        uint32_t at = 0;
+        if (in) at = off[w][d] + (uint32_t)__popcll(same & lanemask_lt());
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (in && (same & lanemask_lt()) == 0) off[w][d] += (uint32_t)__popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (in) {
+            okey[at] = k;
+            opos[at] = pos[b + i + lane];
+        }
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+rows_zero_kernel(T *p, uint64_t count) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (uint64_t)gridDim.x * 256) p[i] = from_f32<T>(0.f);
+}
+
+// grad[row] = (or +=) scale * sum of the row's gradients in order of position. One wave per sorted position; the one
+// that opens a row's run adds the run up.
+template <class T, class O>
+__global__ void __launch_bounds__(256)
+rows_grad_kernel(const T *g, uint64_t stride, const uint32_t *key, const uint32_t *pos, uint32_t t, uint64_t n_rows, uint32_t dim, float scale,
+                 uint32_t accumulate, O *grad) {
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint64_t i = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < t; i += (uint64_t)gridDim.x * 4) {
+        const uint32_t row = key[i];
+        if (row >= n_rows || (i > 0 && key[i - 1] == row)) continue;
+        for (uint32_t e = lane; e < dim; e += 64) {
+            float sum = 0.f;
+            for (uint64_t j = i; j < t && key[j] == row; ++j) sum += to_f32(g[(uint64_t)pos[j] * stride + e]);
+            O *o = grad + (uint64_t)row * dim + e;
+            *o = from_f32<O>(accumulate ? __builtin_fmaf(scale, sum, to_f32(*o)) : scale * sum);
+        }
+    }
+}
+
+} // namespace cuddle

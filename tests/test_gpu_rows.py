@@ -272,7 +272,8 @@ def _check_grad(got, g, ids, n, scale, out, prev=None):
 
 
 @pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32), (F32, BF16), (F16, BF16)])
-@pytest.mark.parametrize("n,d,t", [(1, 1, 1), (1, 64, 300), (10, 33, 5), (50, 128, 2048), (300, 130, 2049), (70_000, 16, 5000), (3, 960, 700), (257, 8, 10_000)])
+@pytest.mark.parametrize("n,d,t", [(1, 1, 1), (1, 64, 300), (10, 33, 5), (50, 128, 2048), (300, 130, 2049), (70_000, 16, 5000), (3, 960, 700), (257, 8, 10_000), (40, 24, 3840), (40, 24, 3841),
+                                   (1_200_000, 4, 140_000), (2, 520, 200_000)])
 def test_rows_grad(gpu, n, d, t, dtype, out):
     rng = np.random.default_rng(n + d + t)
     g = torch.from_numpy(rng.standard_normal((t, d)).astype(np.float32)).to(dtype).cuda(gpu)

@@ -3204,20 +3204,33 @@ extern "C" cuddle_status cuddle_rows_lookup_device(const void *d_table, uint32_t
 }
 
 namespace {
+// Work space of a gradient: sorted keys and places (two of each for more than one pass), tile histograms, the map of
+// named rows, the parts of runs that chunks cut.
 struct GradWs {
-    size_t key[2], pos[2], hist, bytes;
+    uint32_t R = 0, chunks = 0;
+    size_t key[2] = {0, 0}, pos[2] = {0, 0}, hist = 0, total = 0, named = 0, part = 0, bytes = 0;
 };
-GradWs grad_ws(uint64_t n_ids) {
-    GradWs w{};
+GradWs grad_ws(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
+    GradWs w;
     size_t at = 0;
-    for (int i = 0; i < 2; ++i) {
-        w.key[i] = at;
-        at += round_ws(n_ids * 4);
-        w.pos[i] = at;
-        at += round_ws(n_ids * 4);
+    auto take = [&](size_t b) {
+        const size_t p = at;
+        at += round_ws(b);
+        return p;
+    };
+    w.R = n_ids > (128u << 10) ? 32 : n_ids > kSortSmall ? 16 : 8; // enough chunks to fill the chip, few enough cut runs
+    w.chunks = (uint32_t)((n_ids + w.R - 1) / w.R);
+    const bool small = n_ids <= kSortSmall;
+    for (int i = 0; i < (small ? 1 : 2); ++i) {
+        w.key[i] = take(n_ids * 4);
+        w.pos[i] = take(n_ids * 4);
     }
-    w.hist = at;
-    at += round_ws((n_ids + kSortTile - 1) / kSortTile * 1024);
+    if (!small) {
+        w.hist = take(((n_ids + kSortTile - 1) / kSortTile << kSortMaxBits) * 4);
+        w.total = take(4u << kSortMaxBits);
+        w.named = take(n_rows);
+    }
+    w.part = take((size_t)w.chunks * 2 * dim * 4);
     w.bytes = at;
     return w;
 }
@@ -3232,7 +3245,7 @@ cuddle_status check_grad_sizes(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
 extern "C" cuddle_status cuddle_rows_grad_workspace(uint64_t n_ids, uint64_t n_rows, uint32_t dim, uint64_t *bytes) {
     if (!bytes) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
     ST_TRY(check_grad_sizes(n_ids, n_rows, dim));
-    *bytes = grad_ws(n_ids).bytes;
+    *bytes = grad_ws(n_ids, n_rows, dim).bytes;
     return CUDDLE_OK;
 }
 
@@ -3249,42 +3262,91 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
     if (row_stride < dim && n_ids > 1) return fail(CUDDLE_ERR_BAD_ARG, "row_stride %llu < dim %u", (unsigned long long)row_stride, dim);
     ST_TRY(check_elem_align(d_grad_out, type));
     ST_TRY(check_elem_align(d_grad, grad_type));
-    const GradWs w = grad_ws(n_ids);
+    const GradWs w = grad_ws(n_ids, n_rows, dim);
     if (n_ids && n_rows) ST_TRY(check_ws(d_ws, ws_bytes, w.bytes));
     DeviceGuard guard;
     ST_TRY(guard.enter(device_id));
     if (n_rows == 0) return CUDDLE_OK;
     const bool add = flags & CUDDLE_GRAD_ACCUMULATE;
-    if (!add)
-        with_type(grad_type, [&](auto z) {
-            using O = decltype(z);
-            const uint64_t total = n_rows * dim;
-            hipLaunchKernelGGL(rows_zero_kernel<O>, dim3(grid_for((total + 255) / 256)), dim3(256), 0, s, (O *)d_grad, total);
-        });
+    const uint64_t grad_bytes = n_rows * dim * type_size(grad_type);
     if (n_ids == 0) {
+        if (!add) hipLaunchKernelGGL(rows_zero_kernel, dim3(grid_for(grad_bytes / 16384)), dim3(256), 0, s, d_grad, grad_bytes);
         HIP_TRY(hipGetLastError());
         return CUDDLE_OK;
     }
     uint8_t *ws = (uint8_t *)d_ws;
-    uint32_t *key[2] = {(uint32_t *)(ws + w.key[0]), (uint32_t *)(ws + w.key[1])}, *pos[2] = {(uint32_t *)(ws + w.pos[0]), (uint32_t *)(ws + w.pos[1])};
-    uint32_t *hist = (uint32_t *)(ws + w.hist);
-    const uint32_t t = (uint32_t)n_ids, tiles = (t + kSortTile - 1) / kSortTile;
-    with_id(id_bits, [&](auto zi) {
-        using I = decltype(zi);
-        hipLaunchKernelGGL(rows_key_kernel<I>, dim3(grid_for((n_ids + 255) / 256)), dim3(256), 0, s, (const I *)d_ids, n_ids, n_rows, key[0], pos[0]);
-    });
+    const uint32_t t = (uint32_t)n_ids;
+    uint32_t row_bits = 1;
+    while (n_rows >> row_bits) ++row_bits; // keys are 0 .. n_rows
     int cur = 0;
-    for (uint32_t shift = 0; shift < 32 && (n_rows >> shift); shift += 8, cur ^= 1) {
-        hipLaunchKernelGGL(rows_sort_hist_kernel, dim3(tiles), dim3(256), 0, s, key[cur], t, shift, hist);
-        hipLaunchKernelGGL(rows_sort_scan_kernel, dim3(1), dim3(256), 0, s, hist, tiles);
-        hipLaunchKernelGGL(rows_sort_scatter_kernel, dim3(tiles), dim3(256), 0, s, key[cur], pos[cur], t, shift, hist, key[cur ^ 1], pos[cur ^ 1]);
+    uint8_t *named = nullptr;
+    if (t <= kSortSmall) {
+        const unsigned zero_blocks = add ? 0 : (unsigned)std::min<uint64_t>((grad_bytes + 65535) / 65536, 4096);
+        with_id(id_bits, [&](auto zi) {
+            using I = decltype(zi);
+            hipLaunchKernelGGL(rows_sort_small_kernel<I>, dim3(1 + zero_blocks), dim3(1024), 0, s, (const I *)d_ids, t, n_rows, (row_bits + 7) / 8,
+                               (uint32_t *)(ws + w.key[0]), (uint32_t *)(ws + w.pos[0]), d_grad, grad_bytes);
+        });
+    } else {
+        uint32_t *hist = (uint32_t *)(ws + w.hist), *total = (uint32_t *)(ws + w.total);
+        const uint32_t tiles = (t + kSortTile - 1) / kSortTile, passes = (row_bits + kSortMaxBits - 1) / kSortMaxBits, bits = (row_bits + passes - 1) / passes;
+        const unsigned clear = add ? 0 : (unsigned)std::min<uint64_t>((n_rows + 16383) / 16384, 256);
+        named = add ? nullptr : ws + w.named;
+        for (uint32_t p = 0; p < passes; ++p, cur ^= 1) {
+            const uint32_t shift = p * bits;
+            uint32_t *okey = (uint32_t *)(ws + w.key[cur ^ 1]), *opos = (uint32_t *)(ws + w.pos[cur ^ 1]);
+            const uint32_t *ikey = (const uint32_t *)(ws + w.key[cur]), *ipos = (const uint32_t *)(ws + w.pos[cur]);
+            auto scan = [&]() { hipLaunchKernelGGL(rows_sort_scan_kernel, dim3(((1u << bits) + 63) / 64), dim3(1024), 0, s, hist, tiles, 1u << bits, total); };
+            if (p == 0)
+                with_id(id_bits, [&](auto zi) {
+                    using I = decltype(zi);
+                    hipLaunchKernelGGL((rows_sort_hist_kernel<true, I>), dim3(tiles + clear), dim3(256), 0, s, d_ids, t, n_rows, shift, bits, tiles, hist, ws + w.named);
+                    scan();
+                    hipLaunchKernelGGL((rows_sort_scatter_kernel<true, I>), dim3(tiles), dim3(256), 0, s, d_ids, (const uint32_t *)nullptr, t, n_rows, shift, bits, hist,
+                                       total, okey, opos, named);
+                });
+            else {
+                hipLaunchKernelGGL((rows_sort_hist_kernel<false, int32_t>), dim3(tiles), dim3(256), 0, s, (const void *)ikey, t, n_rows, shift, bits, tiles, hist,
+                                   (uint8_t *)nullptr);
+                scan();
+                hipLaunchKernelGGL((rows_sort_scatter_kernel<false, int32_t>), dim3(tiles), dim3(256), 0, s, (const void *)ikey, ipos, t, n_rows, shift, bits, hist, total,
+                                   okey, opos, (uint8_t *)nullptr);
+            }
+        }
     }
+    // Columns per lane: 16 bytes of the gradients where addresses and dim allow, one element otherwise. Lanes per chunk:
+    // the widest group that leaves few of its lanes without a column.
+    const uint32_t ts = type_size(type), os = type_size(grad_type), vmax = 16 / ts;
+    const bool vec = dim % vmax == 0 && aligned16(d_grad_out) && row_stride * ts % 16 == 0 && ((uintptr_t)d_grad & (std::min(vmax * os, 16u) - 1)) == 0;
+    const uint32_t V = vec ? vmax : 1, vpr = dim / V;
+    uint32_t lg = 6;
+    while (lg > 3 && ((vpr + (1u << lg) - 1) >> lg << lg) > vpr + vpr / 8) --lg;
+    GradArgs a;
+    a.key = (const uint32_t *)(ws + w.key[cur]);
+    a.pos = (const uint32_t *)(ws + w.pos[cur]);
+    a.t = t;
+    a.chunks = w.chunks;
+    a.R = w.R;
+    a.lg = lg;
+    a.cbs = (vpr + (1u << lg) - 1) >> lg;
+    const uint64_t blocks = ((uint64_t)w.chunks * a.cbs + (256u >> lg) - 1) / (256u >> lg);
+    if (blocks > kMaxBlocksPerLaunch - 4096) return fail(CUDDLE_ERR_UNSUPPORTED, "n_ids * dim too large");
+    a.blocks = (uint32_t)blocks;
+    a.n_rows = n_rows;
+    a.dim = dim;
+    a.scale = scale;
+    a.accumulate = add ? 1u : 0u;
+    a.part = (float *)(ws + w.part);
+    a.named = named;
+    const unsigned zero_blocks = named ? (unsigned)std::min<uint64_t>((grad_bytes + 16383) / 16384, 4096) : 0;
     with_type(type, [&](auto z) {
         using T = decltype(z);
         with_type(grad_type, [&](auto zo) {
             using O = decltype(zo);
-            hipLaunchKernelGGL((rows_grad_kernel<T, O>), dim3(grid_for((n_ids + 3) / 4)), dim3(256), 0, s, (const T *)d_grad_out, row_stride, key[cur], pos[cur], t,
-                               n_rows, dim, scale, add ? 1u : 0u, (O *)d_grad);
+            auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks + zero_blocks), dim3(256), 0, s, (const T *)d_grad_out, row_stride, a, (O *)d_grad); };
+            if (vec) go(rows_grad_kernel<T, O, 16 / sizeof(T)>);
+            else go(rows_grad_kernel<T, O, 1>);
+            if (a.chunks > 1) hipLaunchKernelGGL(rows_grad_join_kernel<O>, dim3(std::min<uint32_t>(a.chunks - 1, 1u << 16)), dim3(256), 0, s, a, (O *)d_grad);
         });
     });
     HIP_TRY(hipGetLastError());

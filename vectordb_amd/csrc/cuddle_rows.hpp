@@ -508,114 +508,345 @@ int4_topk_none_kernel(uint64_t *ids, float *out, uint32_t *count, uint64_t total
 // ---------------------------------------------------------------------------------------------
 // gradient of the lookup
 // ---------------------------------------------------------------------------------------------
-// Stable radix sort of (row, position) by row, 8 bits per pass: tile histograms, their prefix sums, scatter. Ids
-// outside the table get the key n_rows and end up behind everything.
-constexpr uint32_t kSortTile = 2048;
+// The places (positions in the list of ids) are sorted by row, stably, so that a row's places are neighbours in the
+// order they came in; then each row's run of places is added up. Ids outside the table get the key n_rows, which sorts
+// behind everything and is left out. All of it is integer work until the sums, and the sums' order depends on the
+// sizes alone.
 
+// Key of place i: its row, or n_rows.
 template <class I>
-__global__ void __launch_bounds__(256)
-rows_key_kernel(const I *ids, uint64_t t, uint64_t n_rows, uint32_t *key, uint32_t *pos) {
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < t; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t r = row_of_id(ids, i, n_rows);
-        key[i] = r == kNoRow ? (uint32_t)n_rows : (uint32_t)r;
-        pos[i] = (uint32_t)i;
+__device__ __forceinline__ uint32_t grad_key(const I *ids, uint64_t i, uint64_t n_rows) {
+    const uint64_t r = row_of_id(ids, i, n_rows);
+    return r == kNoRow ? (uint32_t)n_rows : (uint32_t)r;
+}
+
+// A block's share of zeroing `bytes` at p, 16 bytes per store where the address allows.
+__device__ __forceinline__ void zero_share(void *p, uint64_t bytes, uint64_t part, uint64_t parts) {
+    uint8_t *b = static_cast<uint8_t *>(p);
+    const uint64_t head = min(bytes, (uint64_t)(-(intptr_t)b & 15)), vecs = (bytes - head) / 16;
+    uint4 *v = reinterpret_cast<uint4 *>(b + head);
+    for (uint64_t i = part * blockDim.x + threadIdx.x; i < vecs; i += parts * blockDim.x) v[i] = make_uint4(0, 0, 0, 0);
+    if (part == 0) {
+        for (uint64_t i = threadIdx.x; i < head; i += blockDim.x) b[i] = 0;
+        for (uint64_t i = head + vecs * 16 + threadIdx.x; i < bytes; i += blockDim.x) b[i] = 0;
     }
 }
 
 __global__ void __launch_bounds__(256)
-rows_sort_hist_kernel(const uint32_t *key, uint32_t t, uint32_t shift, uint32_t *hist) {
-    __shared__ uint32_t h[256];
-    h[threadIdx.x] = 0;
-    __syncthreads();
-    const uint32_t b = blockIdx.x * kSortTile, e = min(b + kSortTile, t);
-    for (uint32_t i = b + threadIdx.x; i < e; i += 256) atomicAdd(&h[(key[i] >> shift) & 255], 1u);
-    __syncthreads();
-    hist[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
+rows_zero_kernel(void *p, uint64_t bytes) { zero_share(p, bytes, blockIdx.x, gridDim.x); }
+
+// Where 64 neighbouring keys of one wave go: off[digit] (LDS, this wave's own) holds the next place of each digit;
+// lanes with the same digit find each other by one ballot per digit bit, their order is the lane order.
+__device__ __forceinline__ uint32_t wave_rank(uint32_t d, bool in, uint32_t bits, uint32_t *off) {
+    uint64_t same = __ballot(in);
+    for (uint32_t b = 0; b < bits; ++b) {
+        const uint64_t m = __ballot((d >> b) & 1);
+        same &= (d >> b) & 1 ? m : ~m;
+    }
+    const uint64_t below = same & lanemask_lt();
+    const uint32_t at = in ? off[d] + (uint32_t)__popcll(below) : 0u;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); // the reads above, before the update below
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (in && below == 0) off[d] += (uint32_t)__popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    return at;
 }
 
-// hist[tile][digit] -> where the tile's first key of that digit goes. One block of 256 threads, one per digit.
-__global__ void __launch_bounds__(256)
-rows_sort_scan_kernel(uint32_t *hist, uint32_t tiles) {
+// Few places: block 0 sorts them all in LDS, 8 bits per pass, 16 waves with at most 256 keys each; the
+// other blocks zero the gradient meanwhile (zero == nullptr: it is added to). block 1024.
+constexpr uint32_t kSortSmall = 3840; // what 64 KB of LDS hold beside the counters
+template <class I>
+__global__ void __launch_bounds__(1024)
+rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passes, uint32_t *okey, uint32_t *opos, void *zero, uint64_t zero_bytes) {
+    if (blockIdx.x) {
+        zero_share(zero, zero_bytes, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    __shared__ uint32_t key[2][kSortSmall];
+    __shared__ uint16_t pos[2][kSortSmall];
+    __shared__ uint32_t off[16][256];
     __shared__ uint32_t tot[257];
-    const uint32_t d = threadIdx.x;
+    const uint32_t tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    const uint32_t per = (((t + 15) / 16) + 63) & ~63u, b = w * per; // keys of a wave
+    for (uint32_t i = tid; i < t; i += 1024) {
+        key[0][i] = grad_key(ids, i, n_rows);
+        pos[0][i] = (uint16_t)i;
+    }
+    uint32_t cur = 0;
+    for (uint32_t p = 0; p < passes; ++p, cur ^= 1) {
+        const uint32_t shift = 8 * p;
+        for (uint32_t i = tid; i < 16 * 256; i += 1024) (&off[0][0])[i] = 0;
+        __syncthreads();
+        for (uint32_t i = b + lane; i < min(b + per, t); i += 64) atomicAdd(&off[w][(key[cur][i] >> shift) & 255], 1u);
+        __syncthreads();
+        if (tid < 256) {
+            uint32_t run = 0;
+            for (int v = 0; v < 16; ++v) run += off[v][tid];
+            tot[tid] = run;
+        }
+        __syncthreads();
+        wave0_exclusive_scan_lds(tot, 256);
+        __syncthreads();
+        if (tid < 256) {
+            uint32_t run = tot[tid];
+            for (int v = 0; v < 16; ++v) {
+                const uint32_t c = off[v][tid];
+                off[v][tid] = run;
+                run += c;
+            }
+        }
+        __syncthreads();
+        for (uint32_t i0 = b; i0 < b + per; i0 += 64) {
+            const uint32_t i = i0 + lane;
+            const bool in = i < t;
+            const uint32_t k = in ? key[cur][i] : 0u;
+            const uint32_t at = wave_rank((k >> shift) & 255, in, 8, off[w]);
+            if (in) {
+                key[cur ^ 1][at] = k;
+                pos[cur ^ 1][at] = pos[cur][i];
+            }
+        }
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < t; i += 1024) {
+        okey[i] = key[cur][i];
+        opos[i] = pos[cur][i];
+    }
+}
+
+// More places: per pass (up to 10 bits) a histogram per tile of 4096 places, the histograms' prefix sums, the scatter.
+// The first pass reads the ids themselves. The first histogram launch also clears the map of rows that ids name
+// (one byte each), the first scatter fills it in; the gradient kernel zeroes the rows it does not hold.
+constexpr uint32_t kSortTile = 4096, kSortMaxBits = 10;
+
+template <bool FIRST, class I>
+__global__ void __launch_bounds__(256)
+rows_sort_hist_kernel(const void *src, uint32_t t, uint64_t n_rows, uint32_t shift, uint32_t bits, uint32_t tiles, uint32_t *hist, uint8_t *named) {
+    if (blockIdx.x >= tiles) {
+        zero_share(named, n_rows, blockIdx.x - tiles, gridDim.x - tiles);
+        return;
+    }
+    __shared__ uint32_t h[1u << kSortMaxBits];
+    const uint32_t bins = 1u << bits;
+    for (uint32_t i = threadIdx.x; i < bins; i += 256) h[i] = 0;
+    __syncthreads();
+    const uint32_t b = blockIdx.x * kSortTile;
+#pragma unroll
+    for (uint32_t j = 0; j < kSortTile / 256; ++j) {
+        const uint32_t i = b + j * 256 + threadIdx.x;
+        if (i < t) {
+            const uint32_t k = FIRST ? grad_key(static_cast<const I *>(src), i, n_rows) : static_cast<const uint32_t *>(src)[i];
+            atomicAdd(&h[(k >> shift) & (bins - 1)], 1u);
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < bins; i += 256) hist[(uint64_t)blockIdx.x * bins + i] = h[i];
+}
+
+// hist[tile][digit] -> places of that digit in the tiles before; total[digit]. A block has 64 digits, its 16 waves a
+// sixteenth of the tiles each. grid ceil(bins / 64), block 1024.
+__global__ void __launch_bounds__(1024)
+rows_sort_scan_kernel(uint32_t *hist, uint32_t tiles, uint32_t bins, uint32_t *total) {
+    __shared__ uint32_t part[16][64];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
+    const uint32_t per = (tiles + 15) / 16, b = min(w * per, tiles), e = min(b + per, tiles);
+    uint32_t sum = 0;
+    if (d < bins)
+        for (uint32_t i = b; i < e; ++i) sum += hist[(uint64_t)i * bins + d];
+    part[w][lane] = sum;
+    __syncthreads();
     uint32_t run = 0;
-    for (uint32_t i = 0; i < tiles; ++i) run += hist[i * 256 + d];
-    tot[d] = run;
-    __syncthreads();
-    wave0_exclusive_scan_lds(tot, 256);
-    __syncthreads();
-    run = tot[d];
-    for (uint32_t i = 0; i < tiles; ++i) {
-        const uint32_t v = hist[i * 256 + d];
-        hist[i * 256 + d] = run;
+    for (uint32_t v = 0; v < w; ++v) run += part[v][lane];
+    if (d >= bins) return;
+    if (w == 15) total[d] = run + sum;
+    for (uint32_t i = b; i < e; ++i) {
+        const uint32_t v = hist[(uint64_t)i * bins + d];
+        hist[(uint64_t)i * bins + d] = run;
         run += v;
     }
 }
 
-// Each wave ranks its own 512 consecutive keys, 64 at a time: lanes with the same digit find each other by eight ballots.
+template <bool FIRST, class I>
 __global__ void __launch_bounds__(256)
-rows_sort_scatter_kernel(const uint32_t *key, const uint32_t *pos, uint32_t t, uint32_t shift, const uint32_t *hist, uint32_t *okey, uint32_t *opos) {
-    __shared__ uint32_t off[4][256];
-    const uint32_t tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-    for (int v = 0; v < 4; ++v) off[v][tid] = 0;
+rows_sort_scatter_kernel(const void *src, const uint32_t *pos, uint32_t t, uint64_t n_rows, uint32_t shift, uint32_t bits, const uint32_t *hist,
+                         const uint32_t *total, uint32_t *okey, uint32_t *opos, uint8_t *named) {
+    __shared__ uint32_t off[4][1u << kSortMaxBits];
+    __shared__ uint32_t tot[(1u << kSortMaxBits) + 1];
+    const uint32_t tid = threadIdx.x, w = tid >> 6, lane = tid & 63, bins = 1u << bits;
+    for (uint32_t i = tid; i < bins; i += 256) {
+        off[0][i] = off[1][i] = off[2][i] = off[3][i] = 0;
+        tot[i] = total[i];
+    }
     __syncthreads();
     const uint32_t b = blockIdx.x * kSortTile + w * (kSortTile / 4);
-    for (uint32_t i = 0; i < kSortTile / 4; i += 64)
-        if (b + i + lane < t) atomicAdd(&off[w][(key[b + i + lane] >> shift) & 255], 1u);
-    __syncthreads();
-    uint32_t run = hist[blockIdx.x * 256 + tid];
-    for (int v = 0; v < 4; ++v) {
-        const uint32_t c = off[v][tid];
-        off[v][tid] = run;
-        run += c;
-    }
-    __syncthreads();
-    for (uint32_t i = 0; i < kSortTile / 4; i += 64) {
-        const bool in = b + i + lane < t;
-        const uint32_t k = in ? key[b + i + lane] : 0u, d = (k >> shift) & 255;
-        uint64_t same = __ballot(in);
+    uint32_t k[kSortTile / 256], ps[kSortTile / 256];
 #pragma unroll
-        for (int bit = 0; bit < 8; ++bit) {
-            const uint64_t m = __ballot((d >> bit) & 1);
-            same &= (d >> bit) & 1 ? m : ~m;
+    for (uint32_t j = 0; j < kSortTile / 256; ++j) {
+        const uint32_t i = b + j * 64 + lane;
+        const bool in = i < t;
+        k[j] = in ? (FIRST ? grad_key(static_cast<const I *>(src), i, n_rows) : static_cast<const uint32_t *>(src)[i]) : 0u;
+        ps[j] = in ? (FIRST ? i : pos[i]) : 0u;
+        if (in) atomicAdd(&off[w][(k[j] >> shift) & (bins - 1)], 1u);
+        if (FIRST && named && in && k[j] < n_rows) named[k[j]] = 1;
+    }
+    wave0_exclusive_scan_lds(tot, bins);
+    __syncthreads();
+    for (uint32_t i = tid; i < bins; i += 256) {
+        uint32_t run = tot[i] + hist[(uint64_t)blockIdx.x * bins + i];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const uint32_t c = off[v][i];
+            off[v][i] = run;
+            run += c;
         }
-        uint32_t at = 0;
-        if (in) at = off[w][d] + (uint32_t)__popcll(same & lanemask_lt());
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (in && (same & lanemask_lt()) == 0) off[w][d] += (uint32_t)__popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kSortTile / 256; ++j) {
+        const bool in = b + j * 64 + lane < t;
+        const uint32_t at = wave_rank((k[j] >> shift) & (bins - 1), in, bits, off[w]);
         if (in) {
-            okey[at] = k;
-            opos[at] = pos[b + i + lane];
+            okey[at] = k[j];
+            opos[at] = ps[j];
         }
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(256)
-rows_zero_kernel(T *p, uint64_t count) {
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (uint64_t)gridDim.x * 256) p[i] = from_f32<T>(0.f);
+template <class O, int V>
+__device__ __forceinline__ void grad_store(O *o, const float (&sum)[V], float scale, uint32_t accumulate) {
+    Pack<O, V> v;
+    if (accumulate) {
+        v = *reinterpret_cast<const Pack<O, V> *>(o);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v.v[i] = from_f32<O>(__builtin_fmaf(scale, sum[i], to_f32(v.v[i])));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v.v[i] = from_f32<O>(scale * sum[i]);
+    }
+    *reinterpret_cast<Pack<O, V> *>(o) = v;
 }
 
-// grad[row] = (or +=) scale * sum of the row's gradients in order of position. One wave per sorted position; the one
-// that opens a row's run adds the run up.
-template <class T, class O>
+// The sums. The sorted places are cut into chunks of R; L = 1 << lg lanes take one chunk and L * V columns, V columns a
+// lane, and walk the chunk with the rows of U places in flight. A run that lies inside the chunk goes to the gradient;
+// of a run that the chunk's borders cut, the part that opens the run goes to part[2c + 1], a part that continues one to
+// part[2c] (f32, dim columns), and rows_grad_join_kernel adds them up. So no run, however long, is one wave's work.
+// Blocks from `blocks` on zero the rows that no id names. Bound by the read of the gradients, a row at a time, and the
+// write of the table's gradient.
+struct GradArgs {
+    const uint32_t *key, *pos;
+    uint32_t t, chunks, R, lg, cbs, blocks; // cbs: column blocks of L * V
+    uint64_t n_rows;
+    uint32_t dim;
+    float scale;
+    uint32_t accumulate;
+    float *part;
+    const uint8_t *named; // nullptr: nothing to zero here
+};
+
+template <class T, class O, int V>
 __global__ void __launch_bounds__(256)
-rows_grad_kernel(const T *g, uint64_t stride, const uint32_t *key, const uint32_t *pos, uint32_t t, uint64_t n_rows, uint32_t dim, float scale,
-                 uint32_t accumulate, O *grad) {
-    const uint32_t lane = threadIdx.x & 63;
-    for (uint64_t i = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < t; i += (uint64_t)gridDim.x * 4) {
-        const uint32_t row = key[i];
-        if (row >= n_rows || (i > 0 && key[i - 1] == row)) continue;
-        for (uint32_t e = lane; e < dim; e += 64) {
+rows_grad_kernel(const T *g, uint64_t stride, GradArgs a, O *grad) {
+    if (blockIdx.x >= a.blocks) {
+        const uint32_t ppr = a.dim / V, rpb = max(1u, 1024u / ppr); // V divides dim
+        const uint64_t step = (uint64_t)(gridDim.x - a.blocks) * rpb;
+        Pack<O, V> z;
+#pragma unroll
+        for (int i = 0; i < V; ++i) z.v[i] = from_f32<O>(0.f);
+        for (uint64_t r0 = (uint64_t)(blockIdx.x - a.blocks) * rpb; r0 < a.n_rows; r0 += step) {
+            const uint32_t items = (uint32_t)min((uint64_t)rpb, a.n_rows - r0) * ppr;
+            for (uint32_t it = threadIdx.x; it < items; it += 256) {
+                const uint32_t rr = it / ppr, p = it - rr * ppr;
+                if (!a.named[r0 + rr]) *reinterpret_cast<Pack<O, V> *>(grad + (r0 + rr) * a.dim + (uint64_t)p * V) = z;
+            }
+        }
+        return;
+    }
+    const uint32_t L = 1u << a.lg, sub = threadIdx.x & (L - 1);
+    const uint64_t item = ((uint64_t)blockIdx.x << (8 - a.lg)) + (threadIdx.x >> a.lg);
+    const uint32_t c = (uint32_t)(item / a.cbs), cb = (uint32_t)(item % a.cbs);
+    const uint32_t col = (cb * L + sub) * V;
+    if (c >= a.chunks || col >= a.dim) return;
+    const uint32_t begin = c * a.R, end = min(begin + a.R, a.t);
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    uint32_t cur = a.key[begin];
+    bool cont = begin > 0 && a.key[begin - 1] == cur;
+    auto flush = [&](bool open) {
+        if (cur >= a.n_rows) return;
+        if (!cont && !open) {
+            grad_store<O, V>(grad + (uint64_t)cur * a.dim + col, sum, a.scale, a.accumulate);
+        } else {
+            Pack<float, V> v;
+#pragma unroll
+            for (int i = 0; i < V; ++i) v.v[i] = sum[i];
+            *reinterpret_cast<Pack<float, V> *>(a.part + ((uint64_t)c * 2 + (cont ? 0 : 1)) * a.dim + col) = v;
+        }
+    };
+    constexpr int U = 8;
+    for (uint32_t j0 = begin; j0 < end; j0 += U) {
+        uint32_t k[U];
+        Pack<T, V> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t j = min(j0 + u, end - 1);
+            k[u] = a.key[j];
+            v[u] = *reinterpret_cast<const Pack<T, V> *>(g + (uint64_t)a.pos[j] * stride + col);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (j0 + u >= end) break;
+            if (k[u] != cur) {
+                flush(false);
+                cur = k[u];
+                cont = false;
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] += to_f32(v[u].v[i]);
+        }
+    }
+    flush(end < a.t && a.key[end] == cur);
+}
+
+// One block per chunk; it works where a run opens in the chunk and goes on beyond it: the parts of the run, in order, a
+// quarter of them per wave, 64 columns at a time. The last chunk of the run is found by bisection (keys are sorted).
+template <class O>
+__global__ void __launch_bounds__(256)
+rows_grad_join_kernel(GradArgs a, O *grad) {
+    __shared__ float s_part[4][64];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (uint32_t c = blockIdx.x; c + 1 < a.chunks; c += gridDim.x) {
+        const uint32_t begin = c * a.R, end = begin + a.R; // not the last chunk: it is full
+        const uint32_t row = a.key[end - 1];
+        if (row >= a.n_rows || a.key[end] != row) continue;
+        if (a.key[begin] == row && begin > 0 && a.key[begin - 1] == row) continue; // opened earlier
+        uint32_t lo = c + 1, hi = a.chunks - 1; // the last chunk whose first key is the row
+        while (lo < hi) {
+            const uint32_t m = (lo + hi + 1) / 2;
+            if (a.key[m * a.R] == row) lo = m;
+            else hi = m - 1;
+        }
+        const uint32_t parts = lo - c, per = (parts + 3) / 4, p0 = min(w * per, parts), p1 = min(p0 + per, parts);
+        for (uint32_t col0 = 0; col0 < a.dim; col0 += 64) {
+            const uint32_t col = col0 + lane;
             float sum = 0.f;
-            for (uint64_t j = i; j < t && key[j] == row; ++j) sum += to_f32(g[(uint64_t)pos[j] * stride + e]);
-            O *o = grad + (uint64_t)row * dim + e;
-            *o = from_f32<O>(accumulate ? __builtin_fmaf(scale, sum, to_f32(*o)) : scale * sum);
+            if (col < a.dim) {
+                if (w == 0) sum = a.part[((uint64_t)c * 2 + 1) * a.dim + col];
+#pragma unroll 8
+                for (uint32_t p = p0; p < p1; ++p) sum += a.part[(uint64_t)(c + 1 + p) * 2 * a.dim + col];
+            }
+            __syncthreads(); // the sums of the columns before have been read
+            s_part[w][lane] = sum;
+            __syncthreads();
+            if (w == 0 && col < a.dim) {
+                const float one[1] = {((s_part[0][lane] + s_part[1][lane]) + s_part[2][lane]) + s_part[3][lane]};
+                grad_store<O, 1>(grad + (uint64_t)row * a.dim + col, one, a.scale, a.accumulate);
+            }
         }
     }
 }

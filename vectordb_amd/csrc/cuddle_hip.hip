@@ -2997,28 +2997,87 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
     return w;
 }
 
+// Launch shapes of the distance kernel. One quartet of queries: codes are the bound, so many of them are requested at a
+// time (16 pieces of 512 bytes per wave). More: QT quartets per wave, the count among those built that costs least,
+// pairs of (row, query) at about 27 cycles and the unpacking of the codes, once per QT, at about as much.
+constexpr uint32_t kInt4LdsBytes = 64u << 10; // digits per block; two blocks per CU
+
+template <int G, int QT, int T, int P, bool FUSED, class TQ>
+void int4_launch(Int4DistArgs a, hipStream_t s) {
+    a.ku = std::min<uint32_t>((a.units + P - 1) / P * P, kInt4LdsBytes / 1024 / QT / P * P);
+    a.ys = ((a.nq + 3) / 4 + QT - 1) / QT;
+    const uint64_t groups = ((a.n + 15) / 16 + 4 * T - 1) / (4 * T);
+    const size_t lds = (size_t)a.ku * QT * 1024 + QT * 4 * sizeof(Int4Query);
+    uint64_t xs = std::min<uint64_t>(groups, std::max<uint64_t>(64, 2048 / a.ys));
+    if (a.ys > 1) xs = (xs + 7) / 8 * 8;
+    a.xs = (uint32_t)xs;
+    static std::once_flag once[kMaxDevices]; // more than 64 KB of LDS: the kernel's limit is raised, once per device
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    std::call_once(once[dev & (kMaxDevices - 1)], [] {
+        (void)hipFuncSetAttribute((const void *)int4_distance_kernel<G, QT, T, P, FUSED, TQ>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(kInt4LdsBytes + 4096));
+    });
+    hipLaunchKernelGGL((int4_distance_kernel<G, QT, T, P, FUSED, TQ>), dim3((unsigned)(a.xs * a.ys)), dim3(256), lds, s, a);
+}
+
 template <int G>
-void int4_launch_distances(const cuddle_int4_rows *r, const uint8_t *dig, const Int4Query *info, uint32_t nq, uint32_t metric, float *dist, uint64_t dstride,
-                           hipStream_t s) {
-    const uint64_t tiles = (r->n + 15) / 16;
-    constexpr int QT = 1, T = 1;
-    hipLaunchKernelGGL((int4_distance_kernel<G, QT, T>), dim3(grid_for((tiles + 4 * T - 1) / (4 * T)), (nq + 4 * QT - 1) / (4 * QT)), dim3(256), 0, s,
-                       (const uint8_t *)r->codes, (const uint16_t *)r->scales, (const double *)r->sqnorm, r->n, r->dim, dig, info, nq, metric, dist, dstride);
+void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStream_t s) {
+    const uint32_t quads = (a.nq + 3) / 4;
+    const bool few_units = a.units < 6; // short rows: more tiles and fewer units at a time
+    if (fused) {
+        with_type(type, [&](auto z) {
+            using TQ = decltype(z);
+            if (few_units) int4_launch<G, 1, 4, 2, true, TQ>(a, s);
+            else int4_launch<G, 1, 2, 8, true, TQ>(a, s);
+        });
+        return;
+    }
+    uint32_t best = 1, cost = ~0u;
+    for (uint32_t qt : {1u, 2u, 3u, 4u, 6u, 8u}) {
+        const uint32_t ys = (quads + qt - 1) / qt, c = ys * (qt + 1);
+        if (c <= cost) {
+            cost = c;
+            best = qt;
+        }
+    }
+    switch (best) {
+    case 1: int4_launch<G, 1, 2, 8, false, float>(a, s); break;
+    case 2: int4_launch<G, 2, 2, 4, false, float>(a, s); break;
+    case 3: int4_launch<G, 3, 2, 2, false, float>(a, s); break;
+    case 4: int4_launch<G, 4, 2, 2, false, float>(a, s); break;
+    case 6: int4_launch<G, 6, 2, 2, false, float>(a, s); break;
+    default: int4_launch<G, 8, 2, 2, false, float>(a, s); break;
+    }
 }
 
 // Distances of queries [q0, q0 + nq) into dist[q][dstride]; the caller has laid out the work space for nq queries.
 cuddle_status int4_distances_round(const cuddle_int4_rows *r, const void *queries, uint32_t type, uint32_t q0, uint32_t nq, uint32_t metric, float *dist,
                                    uint64_t dstride, uint8_t *ws, const Int4Ws &w, hipStream_t s) {
-    uint8_t *dig = ws + w.dig;
-    Int4Query *info = (Int4Query *)(ws + w.info);
-    const uint32_t units = int4_units(r->dim), padded = (nq + 3) / 4 * 4;
-    with_type(type, [&](auto z) {
-        using T = decltype(z);
-        hipLaunchKernelGGL(int4_query_kernel<T>, dim3(padded), dim3(256), 0, s, (const T *)queries + (uint64_t)q0 * r->dim, nq, r->dim, units, dig, info);
-    });
-    if (r->group == 32) int4_launch_distances<32>(r, dig, info, nq, metric, dist, dstride, s);
-    else if (r->group == 64) int4_launch_distances<64>(r, dig, info, nq, metric, dist, dstride, s);
-    else int4_launch_distances<128>(r, dig, info, nq, metric, dist, dstride, s);
+    Int4DistArgs a{};
+    a.codes = (const uint8_t *)r->codes;
+    a.scales = (const uint16_t *)r->scales;
+    a.sqnorm = (const double *)r->sqnorm;
+    a.n = r->n;
+    a.dim = r->dim;
+    a.units = int4_units(r->dim);
+    a.gs = int4_gstride(r->dim, r->group);
+    a.queries = (const uint8_t *)queries + (uint64_t)q0 * r->dim * type_size(type);
+    a.dig = ws + w.dig;
+    a.info = (const Int4Query *)(ws + w.info);
+    a.nq = nq;
+    a.metric = metric;
+    a.dist = dist;
+    a.dstride = dstride;
+    const bool fused = nq <= 4 && (a.units + 7) / 8 * 8 <= kInt4LdsBytes / 1024;
+    if (!fused)
+        with_type(type, [&](auto z) {
+            using T = decltype(z);
+            hipLaunchKernelGGL(int4_query_kernel<T>, dim3((nq + 3) / 4 * 4), dim3(256), 0, s, (const T *)a.queries, nq, r->dim, a.units, ws + w.dig,
+                               (Int4Query *)(ws + w.info));
+        });
+    if (r->group == 32) int4_launch_group<32>(a, type, fused, s);
+    else if (r->group == 64) int4_launch_group<64>(a, type, fused, s);
+    else int4_launch_group<128>(a, type, fused, s);
     HIP_TRY(hipGetLastError());
     return CUDDLE_OK;
 }

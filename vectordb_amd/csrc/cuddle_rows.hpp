@@ -304,12 +304,6 @@ int4_query_kernel(const T *queries, uint32_t nq, uint32_t dim, uint32_t units, u
     }
 }
 
-// One group's integer products into the running sum: c = the four digits' products of (row r, query h).
-__device__ __forceinline__ double int4_group_sum(double acc, i32x4_t c, double s) {
-    const int32_t lo = c[0] + (c[1] << 8), hi = c[2] + (c[3] << 8);
-    return __builtin_fma(s, __builtin_fma((double)hi, 65536.0, (double)lo), acc);
-}
-
 // distance from the product: l2 |x|^2 + |q|^2 - 2p, cosine 1 - p / (|x||q|), dot -p; in f64, rounded once.
 __device__ __forceinline__ float int4_finish(uint32_t metric, double p, double xsq, double qsq) {
     double d;
@@ -324,74 +318,201 @@ __device__ __forceinline__ float int4_finish(uint32_t metric, double p, double x
     return (float)d;
 }
 
-// One wave: T tiles of 16 rows against QT quartets of queries. Weights are the B operand (a lane has one row), digits the
-// A operand, so that a lane receives the four digits of one (row, query) pair and puts them together itself: per group
-// and pair two integer adds and four f64 operations (f64 runs at the rate of f32 here).
-template <int G, int QT, int T>
-__global__ void __launch_bounds__(256)
-int4_distance_kernel(const uint8_t *codes, const uint16_t *scales, const double *sqnorm, uint64_t n, uint32_t dim, const uint8_t *dig,
-                     const Int4Query *info, uint32_t nq, uint32_t metric, float *dist, uint64_t dstride) {
-    const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
-    const uint32_t units = int4_units(dim), gs = int4_gstride(dim, G);
-    const uint64_t tiles = (n + 15) / 16, groups = (tiles + T - 1) / T;
-    const uint8_t *dg = dig + (uint64_t)blockIdx.y * QT * units * 1024 + lane * 16;
-    for (uint64_t tg = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); tg < groups; tg += (uint64_t)gridDim.x * 4) {
+// The digits of the queries [4 * w] .. of one quartet, made by a block of 256 threads straight into LDS (wave w takes
+// query q0 + w): what int4_query_kernel writes, for blocks that need a single quartet and hold all of it. Units from
+// ceil(dim / 64) to `pad` are zero.
+template <class TQ>
+__device__ __forceinline__ void int4_block_digits(const TQ *queries, uint32_t nq, uint32_t dim, uint32_t pad, uint8_t *dig, Int4Query *info) {
+    const uint32_t q = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const bool real = q < nq;
+    const TQ *src = queries + (uint64_t)(real ? q : 0) * dim;
+    float m = 0.f;
+    double sq = 0.0;
+    if (real)
+        for (uint32_t i = lane; i < dim; i += 64) {
+            const float v = to_f32(src[i]), a = fabsf(v);
+            m = fmaxf(m, a <= 3.4028234663852886e38f ? a : __builtin_huge_valf());
+            sq = __builtin_fma((double)v, (double)v, sq);
+        }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        m = fmaxf(m, __shfl_xor(m, d, 64));
+        sq += __shfl_xor(sq, d, 64);
+    }
+    const bool bad = m > 3.4028234663852886e38f;
+    int e = 0;
+    if (!bad && m > 0.f) (void)frexp((double)m, &e);
+    const double up = ldexp(1.0, 30 - e);
+    if (lane == 0) info[q] = Int4Query{bad ? __builtin_nan("") : ldexp(1.0, e - 34), sq};
+    const uint32_t h = (lane & 31) >> 3, b = ((lane >> 5) << 3) | (lane & 7); // the lane's component of every unit
+    for (uint32_t u = 0; u < pad; ++u) {
+        const uint32_t i = u * 64 + lane;
+        int32_t f = (int32_t)rint((double)(real && i < dim && !bad ? to_f32(src[i]) : 0.f) * up);
+#pragma unroll
+        for (uint32_t d = 0; d < 4; ++d) {
+            const int32_t lo = (int32_t)(int8_t)(f & 255);
+            f = (f - lo) >> 8;
+            dig[u * 1024 + ((h << 4) | (q << 2) | d) * 16 + b] = (uint8_t)lo;
+        }
+    }
+}
+
+// The running sum of one (row, query) pair. The upper two digits' part in f64, the lower two's, 2^-16 of it, in f32:
+// its rounding is 2^-40 of the whole.
+struct Int4Sum {
+    double hi;
+    float lo;
+    __device__ __forceinline__ void add(i32x4_t c, float s) { // c: one group's integer products, digit by digit
+        lo = __builtin_fmaf(s, (float)(c[0] + (c[1] << 8)), lo);
+        hi = __builtin_fma((double)s, (double)(c[2] + (c[3] << 8)), hi);
+    }
+    __device__ __forceinline__ double value() const { return __builtin_fma(hi, 65536.0, (double)lo); }
+};
+
+// W u32 words of a row's scales, 4-byte aligned.
+template <int W> struct __attribute__((packed, aligned(4))) ScaleWords { uint32_t w[W]; };
+
+struct Int4DistArgs {
+    const uint8_t *codes;
+    const uint16_t *scales;
+    const double *sqnorm;
+    uint64_t n;
+    uint32_t dim, units, gs;
+    const void *queries;     // FUSED: the queries themselves
+    const uint8_t *dig;      // otherwise their digits and scalars (int4_query_kernel)
+    const Int4Query *info;
+    uint32_t nq, metric;
+    float *dist;
+    uint64_t dstride;
+    uint32_t ku;             // units of digits in LDS at a time, a multiple of P
+    uint32_t xs, ys;         // blocks along the rows (a multiple of 8 if ys > 1) and along the queries
+};
+
+// Distances. A wave takes T tiles of 16 rows against QT quartets of queries; codes are the B operand (a lane has one
+// row), digits the A operand, so a lane receives the four digits of one (row, query) pair and puts them together itself.
+// The digits sit in LDS, all of them where they fit (loaded, or with FUSED made, once per block: few queries then take
+// one launch), else `ku` units at a time. Codes and scales of P units and T tiles are requested together; units past
+// the end repeat the last one against zero digits.
+// Few queries: bound by the codes' read. Many: by the six vector instructions that a group's products cost per pair
+// (two integer, two conversions, an f32 and an f64 fma; about 27 cycles against 16 of the matrix instruction).
+// Blocks of the same rows and different queries are neighbours on one XCD, so that the rows' codes come from its L2.
+template <int G, int QT, int T, int P, bool FUSED, class TQ>
+__global__ void __launch_bounds__(256, 2) // two waves per SIMD: at most 256 registers, so products land in vector registers, not accumulators
+int4_distance_kernel(Int4DistArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t s_dig[];
+    Int4Query *s_info = reinterpret_cast<Int4Query *>(s_dig + (size_t)a.ku * QT * 1024);
+    const uint32_t tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
+    uint32_t x = blockIdx.x, y = 0;
+    if (a.ys > 1) {
+        const uint32_t j = blockIdx.x >> 3;
+        y = j % a.ys;
+        x = (j / a.ys) * 8 + (blockIdx.x & 7);
+    }
+    const uint64_t tiles = (a.n + 15) / 16, groups = (tiles + 4 * T - 1) / (4 * T);
+    auto load_digits = [&](uint32_t u0) { // digits of units [u0, u0 + ku): [unit][quartet][1 KB]
+        const uint32_t cnt = min(a.ku, a.units - u0), quads = (a.nq + 3) / 4;
+        for (uint32_t i = tid; i < a.ku * QT * 64; i += 256) {
+            const uint32_t u = i / (QT * 64), q = i / 64 % QT, qq = y * QT + q;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (u < cnt && qq < quads) v = reinterpret_cast<const uint4 *>(a.dig)[((uint64_t)qq * a.units + u0 + u) * 64 + (i & 63)];
+            reinterpret_cast<uint4 *>(s_dig)[i] = v;
+        }
+    };
+    if (FUSED)
+        int4_block_digits(static_cast<const TQ *>(a.queries), a.nq, a.dim, a.ku, s_dig, s_info);
+    else {
+        if (tid < QT * 4) s_info[tid] = y * QT * 4 + tid < a.nq ? a.info[y * QT * 4 + tid] : Int4Query{0.0, 0.0};
+        if (a.units <= a.ku) load_digits(0);
+    }
+    __syncthreads();
+    for (uint64_t g = x; g < groups; g += a.xs) {
         const uint8_t *wp[T];
         const uint16_t *sp[T];
-        double acc[T][QT];
+        Int4Sum acc[T][QT];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const uint64_t tile = min(tg * T + t, tiles - 1);
-            wp[t] = codes + tile * units * kInt4UnitBytes + r * 32 + h * 8;
-            sp[t] = scales + min(tile * 16 + r, n - 1) * gs;
+            const uint64_t tile = min((g * 4 + (tid >> 6)) * T + t, tiles - 1);
+            wp[t] = a.codes + tile * a.units * kInt4UnitBytes + r * 32 + h * 8;
+            sp[t] = a.scales + min(tile * 16 + r, a.n - 1) * a.gs;
 #pragma unroll
-            for (int q = 0; q < QT; ++q) acc[t][q] = 0.0;
+            for (int q = 0; q < QT; ++q) acc[t][q] = Int4Sum{0.0, 0.f};
         }
-        i32x4_t c[T][QT];
-        for (uint32_t u = 0; u < units; ++u) {
-            i32x4_t a[QT];
+        for (uint32_t u0 = 0; u0 < a.units; u0 += a.ku) {
+            if (!FUSED && a.units > a.ku) {
+                __syncthreads();
+                load_digits(u0);
+                __syncthreads();
+            }
+            const uint32_t ue = min(u0 + a.ku, a.units);
+            for (uint32_t ub = u0; ub < ue; ub += P) {
+                constexpr int SW = (P * 64 / G + 1) / 2; // words of scales
+                uint2 w[T][P];
+                ScaleWords<SW> sc[T];
 #pragma unroll
-            for (int q = 0; q < QT; ++q) a[q] = *reinterpret_cast<const i32x4_t *>(dg + ((uint64_t)q * units + u) * 1024);
+                for (int t = 0; t < T; ++t) {
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(wp[t] + (uint64_t)u * kInt4UnitBytes);
-                constexpr uint32_t M = 0xF0F0F0F0u;
-                const i32x4_t b = {(int)((w.x << 4) & M), (int)((w.y << 4) & M), (int)(w.x & M), (int)(w.y & M)};
-                const i32x4_t zero = {0, 0, 0, 0};
-                if (G == 32) {
-                    const double s0 = (double)bf16_to_f32(sp[t][2 * u]);
-                    const double s1 = (double)bf16_to_f32(sp[t][2 * u + 1]);
-                    const long b0 = (long)(uint32_t)b[0] | (long)((uint64_t)(uint32_t)b[1] << 32), b1 = (long)(uint32_t)b[2] | (long)((uint64_t)(uint32_t)b[3] << 32);
+                    for (int p = 0; p < P; ++p) w[t][p] = *reinterpret_cast<const uint2 *>(wp[t] + (uint64_t)min(ub + p, a.units - 1) * kInt4UnitBytes);
+                    const uint32_t first = ub * 64 / G; // even: SW words from here are 4-byte aligned (P * 64 / G >= 2, or P = 2 and G = 128)
+                    if (P * 64 / G == 1)
+                        sc[t].w[0] = sp[t][first];
+                    else if (first + 2 * SW <= a.gs)
+                        sc[t] = *reinterpret_cast<const ScaleWords<SW> *>(sp[t] + first);
+                    else {
 #pragma unroll
-                    for (int q = 0; q < QT; ++q) {
-                        const long a0 = (long)(uint32_t)a[q][0] | (long)((uint64_t)(uint32_t)a[q][1] << 32), a1 = (long)(uint32_t)a[q][2] | (long)((uint64_t)(uint32_t)a[q][3] << 32);
-                        acc[t][q] = int4_group_sum(acc[t][q], __builtin_amdgcn_mfma_i32_16x16x32_i8(a0, b0, zero, 0, 0, 0), s0);
-                        acc[t][q] = int4_group_sum(acc[t][q], __builtin_amdgcn_mfma_i32_16x16x32_i8(a1, b1, zero, 0, 0, 0), s1);
+                        for (int i = 0; i < SW; ++i) sc[t].w[i] = *reinterpret_cast<const uint32_t *>(sp[t] + min(first + 2 * i, a.gs - 2));
                     }
-                } else if (G == 64) {
-                    const double s = (double)bf16_to_f32(sp[t][u]);
+                }
+                const i32x4_t zero = {0, 0, 0, 0};
+                constexpr uint32_t M = 0xF0F0F0F0u;
+                constexpr int PP = G == 128 ? 2 : 1; // units per group sum
 #pragma unroll
-                    for (int q = 0; q < QT; ++q) acc[t][q] = int4_group_sum(acc[t][q], __builtin_amdgcn_mfma_i32_16x16x64_i8(a[q], b, zero, 0, 0, 0), s);
-                } else {
+                for (int p0 = 0; p0 < P; p0 += PP) {
+                    i32x4_t dg[PP][QT];
 #pragma unroll
-                    for (int q = 0; q < QT; ++q) c[t][q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[q], b, u & 1 ? c[t][q] : zero, 0, 0, 0);
-                    if ((u & 1) || u + 1 == units) {
-                        const double s = (double)bf16_to_f32(sp[t][u >> 1]);
+                    for (int p = 0; p < PP; ++p)
 #pragma unroll
-                        for (int q = 0; q < QT; ++q) acc[t][q] = int4_group_sum(acc[t][q], c[t][q], s);
+                        for (int q = 0; q < QT; ++q) dg[p][q] = *reinterpret_cast<const i32x4_t *>(s_dig + ((ub - u0 + p0 + p) * QT + q) * 1024 + lane * 16);
+#pragma unroll
+                    for (int t = 0; t < T; ++t) {
+                        i32x4_t b[PP];
+#pragma unroll
+                        for (int p = 0; p < PP; ++p) {
+                            const uint2 v = w[t][p0 + p];
+                            b[p] = i32x4_t{(int)((v.x << 4) & M), (int)((v.y << 4) & M), (int)(v.x & M), (int)(v.y & M)};
+                        }
+                        auto scale = [&](int i) { return __uint_as_float(i & 1 ? sc[t].w[i / 2] & 0xFFFF0000u : sc[t].w[i / 2] << 16); };
+                        if (G == 32) {
+                            auto half = [](i32x4_t v, int i) { return (long)(uint32_t)v[2 * i] | (long)((uint64_t)(uint32_t)v[2 * i + 1] << 32); };
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int q = 0; q < QT; ++q)
+                                    acc[t][q].add(__builtin_amdgcn_mfma_i32_16x16x32_i8(half(dg[0][q], i), half(b[0], i), zero, 0, 0, 0), scale(2 * p0 + i));
+                        } else {
+                            i32x4_t c[QT];
+#pragma unroll
+                            for (int q = 0; q < QT; ++q) c[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(dg[0][q], b[0], zero, 0, 0, 0);
+                            if (PP == 2) {
+#pragma unroll
+                                for (int q = 0; q < QT; ++q) c[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(dg[PP - 1][q], b[PP - 1], c[q], 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int q = 0; q < QT; ++q) acc[t][q].add(c[q], scale(p0 / PP));
+                        }
                     }
                 }
             }
         }
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const uint64_t row = (tg * T + t) * 16 + r;
-            if (row >= n) continue;
-            const double xsq = metric == kMetricDot ? 0.0 : sqnorm[row];
+            const uint64_t row = ((g * 4 + (tid >> 6)) * T + t) * 16 + r;
+            if (row >= a.n) continue;
+            const double xsq = a.metric == kMetricDot ? 0.0 : a.sqnorm[row];
 #pragma unroll
             for (int q = 0; q < QT; ++q) {
-                const uint32_t qi = (blockIdx.y * QT + q) * 4 + h;
-                if (qi < nq) dist[qi * dstride + row] = int4_finish(metric, acc[t][q] * info[qi].scale, xsq, info[qi].sq);
+                const uint32_t qi = (y * QT + q) * 4 + h;
+                const Int4Query qv = s_info[q * 4 + h];
+                if (qi < a.nq) a.dist[qi * a.dstride + row] = int4_finish(a.metric, acc[t][q].value() * qv.scale, xsq, qv.sq);
             }
         }
     }

@@ -538,7 +538,8 @@ typedef enum cuddle_type { CUDDLE_TYPE_F32 = 0, CUDDLE_TYPE_F16 = 1, CUDDLE_TYPE
  *            other; in a block row r has 32 bytes, byte 8h + i (h < 4, i < 8) holding component 8h + i in
  *            its low and 32 + 8h + i in its high nibble, two's complement; components past dim are 0, rows
  *            past n arbitrary. cuddle_int4_sizes gives the bytes. 16-byte aligned.
- *   scales : [n][scale_stride] bf16, scale_stride = ceil(dim / group) rounded up to an even number; 4-byte aligned
+ *   scales : [n][scale_stride] bf16, scale_stride from cuddle_int4_sizes, at least ceil(dim / group), the rest
+ *            of a row 0; 16-byte aligned
  *   sqnorm : [n] f64, |row|^2 of what the row stands for; distances use it (NULL is allowed for DOT and lookups) */
 typedef struct cuddle_int4_rows {
     void *codes;

@@ -170,6 +170,42 @@ def test_search(gpu, n, d, nq, k, metric):
     assert (ids[:, m:] == -1).all() and torch.isinf(got[:, m:]).all()
 
 
+def _check_search(r, q, k, metric):
+    d = r.distances_device(q, metric)
+    ids, got, count = r.search_batch_device(q, k, metric)
+    order = torch.argsort(d, dim=1, stable=True)[:, :k]  # NaN last, equal ones by row
+    assert torch.equal(ids, order)
+    assert np.array_equal(_np(got), _np(torch.gather(d, 1, order)), equal_nan=True)
+    assert count.tolist() == [k] * q.shape[0]
+
+
+@pytest.mark.parametrize("n,nq,k,metric", [(300_007, 128, 10, "l2"), (1_000_001, 36, 1, "cosine"), (600_000, 64, 100, "dot"), (9_000_000, 4, 33, "l2"),
+                                           (300_000, 130, 1024, "l2")])
+def test_search_by_sample(gpu, n, nq, k, metric):
+    """So many distances that the answer comes from a sampled bound and a collection (k = 1024: not sampled)."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(n)
+    x = torch.randn((n, 16), generator=gen, device="cuda")
+    x = x[torch.argsort(x[:, 0])].contiguous()  # an order that a plain prefix would be misled by
+    _check_search(R.int4_encode_device(x, 32), torch.randn((nq, 16), generator=gen, device="cuda"), k, metric)
+
+
+def test_search_by_sample_overflow_ties_nan(gpu):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(3)
+    n = 300_000
+    few = torch.randn((40, 16), generator=gen, device="cuda")
+    x = few[torch.randint(0, 40, (n,), generator=gen, device="cuda")].contiguous()  # 7500 rows each: the bound's ties alone fill the collection
+    q = torch.randn((120, 16), generator=gen, device="cuda")
+    q[5] = float("nan")   # every row ties
+    q[6] = 0.0
+    _check_search(R.int4_encode_device(x, 32), q, 50, "l2")
+    _check_search(R.int4_encode_device(x, 32), q, 50, "dot")
+    x = torch.randn((n, 16), generator=gen, device="cuda")
+    x[torch.rand((n,), generator=gen, device="cuda") < 0.9999] = float("nan")  # about 30 rows with a distance, 100 asked for
+    _check_search(R.int4_encode_device(x, 32), q, 100, "l2")
+
+
 def test_search_ties_nan_and_host_forms(gpu):
     x = np.tile(clustered(50, 40, 5, 1), (400, 1))  # 20 000 rows, every one 400 times
     x[11::50] = np.nan

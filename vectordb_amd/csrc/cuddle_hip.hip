@@ -8,6 +8,7 @@
 #include <dlfcn.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -2937,7 +2938,7 @@ cuddle_status check_rows(const cuddle_int4_rows *r, bool need_sq) {
     ST_TRY(check_group(r->group));
     if (r->n >= 0xFFFFFFFFull) return fail(CUDDLE_ERR_UNSUPPORTED, "%llu rows: fewer than 2^32 - 1", (unsigned long long)r->n);
     if (r->n && (!r->codes || !r->scales || (need_sq && !r->sqnorm))) return fail(CUDDLE_ERR_BAD_ARG, "null pointer");
-    if (!aligned16(r->codes) || ((uintptr_t)r->scales & 3) || ((uintptr_t)r->sqnorm & 7)) return fail(CUDDLE_ERR_BAD_ARG, "codes, scales and sqnorm need alignments of 16, 4 and 8 bytes");
+    if (!aligned16(r->codes) || !aligned16(r->scales) || ((uintptr_t)r->sqnorm & 7)) return fail(CUDDLE_ERR_BAD_ARG, "codes, scales and sqnorm need alignments of 16, 16 and 8 bytes");
     return CUDDLE_OK;
 }
 cuddle_status check_ids(const void *ids, uint32_t id_bits) {
@@ -2966,31 +2967,45 @@ size_t round_ws(size_t b) { return (b + kAlign - 1) & ~(kAlign - 1); }
 // Work space of the distance and search calls: the queries' digits, and for a search the distances of `qc` queries and
 // two selection buffers.
 struct Int4Ws {
-    uint32_t qc = 0; // queries per round
-    size_t dig = 0, info = 0, dist = 0, sel[2] = {0, 0}, bytes = 0;
+    uint32_t qc = 0;     // queries per round
+    uint32_t stride = 0; // 0, or the search samples one tile out of `stride` and collects candidates
+    uint64_t stiles = 0;
+    size_t dig = 0, info = 0, dist = 0, sel[2] = {0, 0}, tau = 0, cnt = 0, list = 0, bytes = 0;
 };
 constexpr uint64_t kInt4DistBudget = 512ull << 20; // bytes of distances a search holds at a time (one quartet of queries at least)
 constexpr uint64_t kInt4MaxRound = 32768;          // queries per round (the launches' second grid dimension)
+// Sampling pays from about this many distances on (they are 128 MB to write and read again; the collection's extra
+// launches cost about 30 us).
+constexpr uint64_t kInt4SampleFrom = 32ull << 20;
 
 Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
     Int4Ws w;
     uint64_t qc = std::min<uint64_t>(nq, kInt4MaxRound);
     if (k) qc = std::min<uint64_t>(qc, std::max<uint64_t>(4, kInt4DistBudget / (std::max<uint64_t>(n, 1) * 4) & ~3ull));
     w.qc = (uint32_t)qc;
-    const uint64_t quartets = (qc + 3) / 4, parts = (n + kTopChunk - 1) / kTopChunk;
+    const uint64_t quartets = (qc + 3) / 4, parts = (n + kTopChunk - 1) / kTopChunk, tiles = (n + 15) / 16;
     size_t at = 0;
-    w.dig = at;
-    at += round_ws(quartets * int4_units(dim) * 1024);
-    w.info = at;
-    at += round_ws(quartets * 4 * sizeof(Int4Query));
+    auto take = [&](size_t b) {
+        const size_t p = at;
+        at += round_ws(b);
+        return p;
+    };
+    w.dig = take(quartets * int4_units(dim) * 1024);
+    w.info = take(quartets * 4 * sizeof(Int4Query));
     if (k) {
-        w.dist = at;
-        at += round_ws((size_t)qc * n * 4);
+        w.dist = take((size_t)qc * n * 4);
         if (parts > 1) {
-            w.sel[0] = at;
-            at += round_ws((size_t)qc * parts * k * 8);
-            w.sel[1] = at;
-            at += round_ws((size_t)qc * ((parts * k + kTopChunk - 1) / kTopChunk) * k * 8);
+            w.sel[0] = take((size_t)qc * parts * k * 8);
+            w.sel[1] = take((size_t)qc * ((parts * k + kTopChunk - 1) / kTopChunk) * k * 8);
+        }
+        // a sample of 4096 rows, or as many as leave half of the collection's room expected to be filled
+        const uint64_t want = std::max<uint64_t>(256, (k * n / (kTopChunk / 2) + 15) / 16);
+        if (qc * n >= kInt4SampleFrom && tiles / want >= 8) {
+            w.stride = (uint32_t)(tiles / want);
+            w.stiles = tiles / w.stride;
+            w.tau = take(qc * 4);
+            w.cnt = take(qc * 4);
+            w.list = take((size_t)qc * kTopChunk * 8);
         }
     }
     w.bytes = at;
@@ -3000,24 +3015,41 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
 // Launch shapes of the distance kernel. One quartet of queries: codes are the bound, so many of them are requested at a
 // time (16 pieces of 512 bytes per wave). More: QT quartets per wave, the count among those built that costs least,
 // pairs of (row, query) at about 27 cycles and the unpacking of the codes, once per QT, at about as much.
-constexpr uint32_t kInt4LdsBytes = 64u << 10; // digits per block; two blocks per CU
+constexpr uint32_t int4_lds_kb(int qt) { return qt >= 3 ? 150u : 64u; } // digits per block: one block of 8 waves per CU, or two of 4 and more
 
-template <int G, int QT, int T, int P, bool FUSED, class TQ>
+template <int G, int QT, int T, int P, bool FUSED, bool NT, class TQ>
 void int4_launch(Int4DistArgs a, hipStream_t s) {
-    a.ku = std::min<uint32_t>((a.units + P - 1) / P * P, kInt4LdsBytes / 1024 / QT / P * P);
+    constexpr uint32_t NW = int4_block(QT) / 64;
+    a.ku = std::min<uint32_t>((a.units + P - 1) / P * P, int4_lds_kb(QT) / QT / P * P);
     a.ys = ((a.nq + 3) / 4 + QT - 1) / QT;
-    const uint64_t groups = ((a.n + 15) / 16 + 4 * T - 1) / (4 * T);
-    const size_t lds = (size_t)a.ku * QT * 1024 + QT * 4 * sizeof(Int4Query);
-    uint64_t xs = std::min<uint64_t>(groups, std::max<uint64_t>(64, 2048 / a.ys));
-    if (a.ys > 1) xs = (xs + 7) / 8 * 8;
-    a.xs = (uint32_t)xs;
+    const uint64_t groups = (a.stiles + NW * T - 1) / (NW * T);
+    const size_t lds = (size_t)a.ku * QT * 1024 + QT * 4 * (sizeof(Int4Query) + 4);
+    static_assert(P * 64 % G == 0, "whole groups");
+    const void *kernel = (const void *)int4_distance_kernel<G, QT, T, P, FUSED, NT, TQ>;
     static std::once_flag once[kMaxDevices]; // more than 64 KB of LDS: the kernel's limit is raised, once per device
     int dev = 0;
     (void)hipGetDevice(&dev);
-    std::call_once(once[dev & (kMaxDevices - 1)], [] {
-        (void)hipFuncSetAttribute((const void *)int4_distance_kernel<G, QT, T, P, FUSED, TQ>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(kInt4LdsBytes + 4096));
+    std::call_once(once[dev & (kMaxDevices - 1)], [kernel] {
+        (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(int4_lds_kb(QT) * 1024 + QT * 4 * (sizeof(Int4Query) + 4)));
     });
-    hipLaunchKernelGGL((int4_distance_kernel<G, QT, T, P, FUSED, TQ>), dim3((unsigned)(a.xs * a.ys)), dim3(256), lds, s, a);
+    // As many blocks as the chip holds at a time, each walking over the rows: blocks per CU of this kernel and LDS size
+    static std::atomic<uint64_t> known{0}; // (lds << 32 | blocks), what the last call asked about
+    uint64_t k = known.load(std::memory_order_relaxed);
+    if (k >> 32 != lds) {
+        int n = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, int4_block(QT), lds) != hipSuccess || n < 1) {
+            (void)hipGetLastError();
+            n = 1;
+        }
+        k = (uint64_t)lds << 32 | (uint32_t)n;
+        known.store(k, std::memory_order_relaxed);
+    }
+    uint64_t xs = std::max<uint64_t>(8, 256 * (uint32_t)k / a.ys);
+    if (a.ys > 1) xs = xs / 8 * 8;
+    xs = std::min<uint64_t>(groups, xs);
+    if (a.ys > 1) xs = (xs + 7) / 8 * 8;
+    a.xs = (uint32_t)xs;
+    hipLaunchKernelGGL((int4_distance_kernel<G, QT, T, P, FUSED, NT, TQ>), dim3((unsigned)(a.xs * a.ys)), dim3(int4_block(QT)), lds, s, a);
 }
 
 template <int G>
@@ -3027,32 +3059,41 @@ void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStre
     if (fused) {
         with_type(type, [&](auto z) {
             using TQ = decltype(z);
-            if (few_units) int4_launch<G, 1, 4, 2, true, TQ>(a, s);
-            else int4_launch<G, 1, 2, 8, true, TQ>(a, s);
+            // beyond the Infinity Cache (256 MB) nothing of the codes is left for the next call
+            const bool nt = (a.n + 15) / 16 * a.units * kInt4UnitBytes > (256ull << 20) && !a.stride;
+            if (few_units && nt) int4_launch<G, 1, 4, 2, true, true, TQ>(a, s);
+            else if (few_units) int4_launch<G, 1, 4, 2, true, false, TQ>(a, s);
+            else if (nt) int4_launch<G, 1, 2, G == 32 ? 4 : 8, true, true, TQ>(a, s);
+            else int4_launch<G, 1, 2, G == 32 ? 4 : 8, true, false, TQ>(a, s);
         });
         return;
     }
     uint32_t best = 1, cost = ~0u;
+    static const char *force = getenv("CUDDLE_QT");
     for (uint32_t qt : {1u, 2u, 3u, 4u, 6u, 8u}) {
-        const uint32_t ys = (quads + qt - 1) / qt, c = ys * (qt + 1);
+        if (force && (uint32_t)atoi(force) != qt) continue;
+        const uint32_t ys = (quads + qt - 1) / qt;
+        const bool whole = a.units <= int4_lds_kb((int)qt) / qt; // else the digits are fetched anew for every 256 rows: about as much again
+        const uint32_t c = ys * (qt * (whole ? 1 : 2) + 1);
         if (c <= cost) {
             cost = c;
             best = qt;
         }
     }
     switch (best) {
-    case 1: int4_launch<G, 1, 2, 8, false, float>(a, s); break;
-    case 2: int4_launch<G, 2, 2, 4, false, float>(a, s); break;
-    case 3: int4_launch<G, 3, 2, 2, false, float>(a, s); break;
-    case 4: int4_launch<G, 4, 2, 2, false, float>(a, s); break;
-    case 6: int4_launch<G, 6, 2, 2, false, float>(a, s); break;
-    default: int4_launch<G, 8, 2, 2, false, float>(a, s); break;
+    case 1: int4_launch<G, 1, 4, 2, false, false, float>(a, s); break;
+    case 2: int4_launch<G, 2, 2, 2, false, false, float>(a, s); break;
+    case 3: int4_launch<G, 3, 2, 2, false, false, float>(a, s); break;
+    case 4: int4_launch<G, 4, 2, 2, false, false, float>(a, s); break;
+    case 6: int4_launch<G, 6, 2, 2, false, false, float>(a, s); break;
+    default: int4_launch<G, 8, 2, 2, false, false, float>(a, s); break;
     }
 }
 
-// Distances of queries [q0, q0 + nq) into dist[q][dstride]; the caller has laid out the work space for nq queries.
-cuddle_status int4_distances_round(const cuddle_int4_rows *r, const void *queries, uint32_t type, uint32_t q0, uint32_t nq, uint32_t metric, float *dist,
-                                   uint64_t dstride, uint8_t *ws, const Int4Ws &w, hipStream_t s) {
+// The distance kernel's arguments for queries [q0, q0 + nq), and their digits enqueued where the kernel does not make
+// them itself; the caller has laid out the work space for nq queries.
+Int4DistArgs int4_prepare(const cuddle_int4_rows *r, const void *queries, uint32_t type, uint32_t q0, uint32_t nq, uint32_t metric, uint8_t *ws, const Int4Ws &w,
+                          bool &fused, hipStream_t s) {
     Int4DistArgs a{};
     a.codes = (const uint8_t *)r->codes;
     a.scales = (const uint16_t *)r->scales;
@@ -3066,20 +3107,21 @@ cuddle_status int4_distances_round(const cuddle_int4_rows *r, const void *querie
     a.info = (const Int4Query *)(ws + w.info);
     a.nq = nq;
     a.metric = metric;
-    a.dist = dist;
-    a.dstride = dstride;
-    const bool fused = nq <= 4 && (a.units + 7) / 8 * 8 <= kInt4LdsBytes / 1024;
+    a.stiles = (r->n + 15) / 16;
+    fused = nq <= 4 && (a.units + 7) / 8 * 8 <= int4_lds_kb(1);
     if (!fused)
         with_type(type, [&](auto z) {
             using T = decltype(z);
             hipLaunchKernelGGL(int4_query_kernel<T>, dim3((nq + 3) / 4 * 4), dim3(256), 0, s, (const T *)a.queries, nq, r->dim, a.units, ws + w.dig,
                                (Int4Query *)(ws + w.info));
         });
-    if (r->group == 32) int4_launch_group<32>(a, type, fused, s);
-    else if (r->group == 64) int4_launch_group<64>(a, type, fused, s);
+    return a;
+}
+
+void int4_run(const Int4DistArgs &a, uint32_t group, uint32_t type, bool fused, hipStream_t s) {
+    if (group == 32) int4_launch_group<32>(a, type, fused, s);
+    else if (group == 64) int4_launch_group<64>(a, type, fused, s);
     else int4_launch_group<128>(a, type, fused, s);
-    HIP_TRY(hipGetLastError());
-    return CUDDLE_OK;
 }
 
 cuddle_status check_query_call(const cuddle_int4_rows *r, const void *queries, uint32_t type, uint32_t nq, uint32_t metric) {
@@ -3179,9 +3221,14 @@ extern "C" cuddle_status cuddle_int4_distances_device(const cuddle_int4_rows *ro
     DeviceGuard guard;
     ST_TRY(guard.enter(device_id));
     if (n_queries == 0 || rows->n == 0) return CUDDLE_OK;
-    for (uint32_t q0 = 0; q0 < n_queries; q0 += w.qc)
-        ST_TRY(int4_distances_round(rows, d_queries, type, q0, std::min(w.qc, n_queries - q0), metric, d_dist + (uint64_t)q0 * rows->n, rows->n, (uint8_t *)d_ws, w,
-                                    (hipStream_t)stream_));
+    for (uint32_t q0 = 0; q0 < n_queries; q0 += w.qc) {
+        bool fused;
+        Int4DistArgs a = int4_prepare(rows, d_queries, type, q0, std::min(w.qc, n_queries - q0), metric, (uint8_t *)d_ws, w, fused, (hipStream_t)stream_);
+        a.dist = d_dist + (uint64_t)q0 * rows->n;
+        a.dstride = rows->n;
+        int4_run(a, rows->group, type, fused, (hipStream_t)stream_);
+        HIP_TRY(hipGetLastError());
+    }
     return CUDDLE_OK;
 }
 
@@ -3209,23 +3256,56 @@ extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows,
     const uint32_t found = (uint32_t)std::min<uint64_t>(k, rows->n);
     for (uint32_t q0 = 0; q0 < n_queries; q0 += w.qc) {
         const uint32_t nq = std::min(w.qc, n_queries - q0);
-        ST_TRY(int4_distances_round(rows, d_queries, type, q0, nq, metric, dist, rows->n, ws, w, s));
+        uint64_t *ids = d_out_ids + (uint64_t)q0 * k;
+        float *od = d_out_dist + (uint64_t)q0 * k;
+        uint32_t *oc = d_out_count ? d_out_count + q0 : nullptr;
+        bool fused;
+        const Int4DistArgs all = int4_prepare(rows, d_queries, type, q0, nq, metric, ws, w, fused, s);
+        uint32_t *cnt = nullptr; // sampled: the candidate counts, by which the levels below know what is left to them
+        if (w.stride && nq * rows->n >= kInt4SampleFrom) { // a last round of few queries takes the levels
+            cnt = (uint32_t *)(ws + w.cnt);
+            uint32_t *tau = (uint32_t *)(ws + w.tau);
+            Int4DistArgs a = all;
+            a.dist = dist;
+            a.dstride = w.stiles * 16;
+            a.stride = w.stride;
+            a.stiles = w.stiles;
+            int4_run(a, rows->group, type, fused, s);
+            hipLaunchKernelGGL(int4_topk_bound_kernel, dim3(nq), dim3(kTopThreads), 0, s, dist, a.dstride, (uint32_t)(w.stiles * 16), k, tau, cnt);
+            a = all;
+            a.tau = tau;
+            a.cnt = cnt;
+            a.list = (uint64_t *)(ws + w.list);
+            a.cap = kTopChunk;
+            int4_run(a, rows->group, type, fused, s);
+            hipLaunchKernelGGL(int4_topk_final_kernel<2>, dim3(nq), dim3(kTopThreads), 0, s, (const void *)a.list, (uint64_t)kTopChunk, 0u, k, found, (const uint32_t *)cnt,
+                               kTopChunk, ids, od, oc);
+        }
+        Int4DistArgs a = all;
+        a.dist = dist;
+        a.dstride = rows->n;
+        a.redo = cnt;
+        a.cap = kTopChunk;
+        int4_run(a, rows->group, type, fused, s);
         const void *in = dist;
         uint64_t stride = rows->n, items = rows->n;
         int level = 0;
         for (; items > kTopChunk; ++level) {
             const uint64_t parts = (items + kTopChunk - 1) / kTopChunk;
             uint64_t *out = (uint64_t *)(ws + w.sel[level & 1]);
-            if (level == 0) hipLaunchKernelGGL(int4_topk_level_kernel<true>, dim3((unsigned)parts, nq), dim3(256), 0, s, in, stride, items, k, out);
-            else hipLaunchKernelGGL(int4_topk_level_kernel<false>, dim3((unsigned)parts, nq), dim3(256), 0, s, in, stride, items, k, out);
+            auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3((unsigned)parts, nq), dim3(kTopThreads), 0, s, in, stride, items, k, out, (const uint32_t *)cnt, kTopChunk);
+            };
+            if (level == 0) go(int4_topk_level_kernel<true>);
+            else go(int4_topk_level_kernel<false>);
             in = out;
             stride = items = parts * k;
         }
-        uint64_t *ids = d_out_ids + (uint64_t)q0 * k;
-        float *od = d_out_dist + (uint64_t)q0 * k;
-        uint32_t *oc = d_out_count ? d_out_count + q0 : nullptr;
-        if (level == 0) hipLaunchKernelGGL(int4_topk_final_kernel<true>, dim3(nq), dim3(256), 0, s, in, stride, (uint32_t)items, k, found, dist, rows->n, ids, od, oc);
-        else hipLaunchKernelGGL(int4_topk_final_kernel<false>, dim3(nq), dim3(256), 0, s, in, stride, (uint32_t)items, k, found, dist, rows->n, ids, od, oc);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(nq), dim3(kTopThreads), 0, s, in, stride, (uint32_t)items, k, found, (const uint32_t *)cnt, kTopChunk, ids, od, oc);
+        };
+        if (level == 0) go(int4_topk_final_kernel<0>);
+        else go(int4_topk_final_kernel<1>);
         HIP_TRY(hipGetLastError());
     }
     return CUDDLE_OK;

@@ -14,7 +14,8 @@
 //   byte h * 8 + i of a row's unit = component 8h + i in the low nibble, 32 + 8h + i in the high nibble (i < 8),
 // two's complement. A wave reads 8 bytes per lane, 512 contiguous bytes, and has both halves of the operand after a
 // shift and two masks; the code stays in the high nibble of its byte, so the products come out 16 times too large
-// (an exact factor, taken out at the end). Scales are row-major: [rows][gstride] bf16, gstride even.
+// (an exact factor, taken out at the end). Scales are row-major: [rows][gstride] bf16; gstride is the number of groups
+// rounded up to 2, 4 or 8, so that the scales of neighbouring units come in one aligned load.
 #pragma once
 
 #include "cuddle_kernels.hpp"
@@ -29,7 +30,8 @@ constexpr uint32_t kInt4UnitBytes = 512; // 16 rows x 32 bytes
 
 __host__ __device__ __forceinline__ uint32_t int4_units(uint32_t dim) { return (dim + kInt4Unit - 1) / kInt4Unit; }
 __host__ __device__ __forceinline__ uint32_t int4_gstride(uint32_t dim, uint32_t group) {
-    return ((dim + group - 1) / group + 1) & ~1u;
+    const uint32_t groups = (dim + group - 1) / group, m = groups > 4 ? 8 : groups > 2 || group == 32 ? 4 : 2;
+    return (groups + m - 1) / m * m;
 }
 
 // ---- element types ---------------------------------------------------------------------------
@@ -164,8 +166,11 @@ int4_encode_kernel(const T *x, uint64_t stride, uint64_t first, uint64_t count, 
                 if (e0 % group == 0 && g < gs) scales[row * gs + g] = sb;
             }
         }
-        // a padding group of the scales' row that no lane above stands for
-        if (act && lane16 == 0 && (uint64_t)(gs - 1) * group >= (uint64_t)units * kInt4Unit) scales[row * gs + gs - 1] = 0;
+        // padding groups of the scales' row that no lane above stands for
+        if (act && lane16 < 8) {
+            const uint32_t g = (units * kInt4Unit + group - 1) / group + lane16;
+            if (g < gs) scales[row * gs + g] = 0;
+        }
 #pragma unroll
         for (int m = 1; m < 16; m <<= 1) sq += __shfl_xor(sq, m, 64);
         if (act && lane16 == 0) sqnorm[row] = sq;
@@ -304,18 +309,12 @@ int4_query_kernel(const T *queries, uint32_t nq, uint32_t dim, uint32_t units, u
     }
 }
 
-// distance from the product: l2 |x|^2 + |q|^2 - 2p, cosine 1 - p / (|x||q|), dot -p; in f64, rounded once.
-__device__ __forceinline__ float int4_finish(uint32_t metric, double p, double xsq, double qsq) {
-    double d;
-    if (metric == kMetricDot)
-        d = -p;
-    else if (metric == kMetricCosine)
-        d = 1.0 - p / (sqrt(xsq) * sqrt(qsq));
-    else {
-        d = (xsq + qsq) - 2.0 * p;
-        d = d < 0.0 ? 0.0 : d; // the three terms of a row next to the query round apart
-    }
-    return (float)d;
+// distance from the product p = scale * sum: l2 |x|^2 + |q|^2 - 2p, cosine 1 - p / (|x||q|), dot -p; in f64, rounded once.
+__device__ __forceinline__ float int4_finish(uint32_t metric, double sum, double scale, double xsq, double qsq) {
+    if (metric == kMetricDot) return (float)(-scale * sum);
+    if (metric == kMetricCosine) return (float)(1.0 - scale * sum / (sqrt(xsq) * sqrt(qsq)));
+    const float d = (float)__builtin_fma(-2.0 * scale, sum, xsq + qsq);
+    return d < 0.f ? 0.f : d; // the three terms of a row next to the query round apart
 }
 
 // The digits of the queries [4 * w] .. of one quartet, made by a block of 256 threads straight into LDS (wave w takes
@@ -328,12 +327,24 @@ __device__ __forceinline__ void int4_block_digits(const TQ *queries, uint32_t nq
     const TQ *src = queries + (uint64_t)(real ? q : 0) * dim;
     float m = 0.f;
     double sq = 0.0;
-    if (real)
-        for (uint32_t i = lane; i < dim; i += 64) {
-            const float v = to_f32(src[i]), a = fabsf(v);
-            m = fmaxf(m, a <= 3.4028234663852886e38f ? a : __builtin_huge_valf());
-            sq = __builtin_fma((double)v, (double)v, sq);
+    constexpr int U = 8; // units read at a time
+    auto read8 = [&](uint32_t u0, float (&v)[U]) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const uint32_t i = (u0 + j) * 64 + lane;
+            v[j] = real && i < dim ? to_f32(src[min(i, dim - 1)]) : 0.f;
         }
+    };
+    for (uint32_t u0 = 0; u0 * 64 < dim; u0 += U) {
+        float v[U];
+        read8(u0, v);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const float a = fabsf(v[j]);
+            m = fmaxf(m, a <= 3.4028234663852886e38f ? a : __builtin_huge_valf());
+            sq = __builtin_fma((double)v[j], (double)v[j], sq);
+        }
+    }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         m = fmaxf(m, __shfl_xor(m, d, 64));
@@ -345,14 +356,19 @@ __device__ __forceinline__ void int4_block_digits(const TQ *queries, uint32_t nq
     const double up = ldexp(1.0, 30 - e);
     if (lane == 0) info[q] = Int4Query{bad ? __builtin_nan("") : ldexp(1.0, e - 34), sq};
     const uint32_t h = (lane & 31) >> 3, b = ((lane >> 5) << 3) | (lane & 7); // the lane's component of every unit
-    for (uint32_t u = 0; u < pad; ++u) {
-        const uint32_t i = u * 64 + lane;
-        int32_t f = (int32_t)rint((double)(real && i < dim && !bad ? to_f32(src[i]) : 0.f) * up);
+    for (uint32_t u0 = 0; u0 < pad; u0 += U) {
+        float v[U];
+        read8(u0, v);
 #pragma unroll
-        for (uint32_t d = 0; d < 4; ++d) {
-            const int32_t lo = (int32_t)(int8_t)(f & 255);
-            f = (f - lo) >> 8;
-            dig[u * 1024 + ((h << 4) | (q << 2) | d) * 16 + b] = (uint8_t)lo;
+        for (int j = 0; j < U; ++j) {
+            if (u0 + j >= pad) break;
+            int32_t f = (int32_t)rint((double)(bad ? 0.f : v[j]) * up);
+#pragma unroll
+            for (uint32_t d = 0; d < 4; ++d) {
+                const int32_t lo = (int32_t)(int8_t)(f & 255);
+                f = (f - lo) >> 8;
+                dig[(u0 + j) * 1024 + ((h << 4) | (q << 2) | d) * 16 + b] = (uint8_t)lo;
+            }
         }
     }
 }
@@ -369,8 +385,7 @@ struct Int4Sum {
     __device__ __forceinline__ double value() const { return __builtin_fma(hi, 65536.0, (double)lo); }
 };
 
-// W u32 words of a row's scales, 4-byte aligned.
-template <int W> struct __attribute__((packed, aligned(4))) ScaleWords { uint32_t w[W]; };
+__host__ __device__ constexpr int int4_block(int qt) { return qt >= 3 ? 512 : 256; } // threads
 
 struct Int4DistArgs {
     const uint8_t *codes;
@@ -386,7 +401,26 @@ struct Int4DistArgs {
     uint64_t dstride;
     uint32_t ku;             // units of digits in LDS at a time, a multiple of P
     uint32_t xs, ys;         // blocks along the rows (a multiple of 8 if ys > 1) and along the queries
+    // search: either a sample of the tiles (dist[q][16 i + r] = row r of the i-th sampled tile, NaN past the last row) ...
+    uint64_t stiles;         // tiles to visit: all, or the sample
+    uint32_t stride;         // 0, or a sampled tile out of every `stride`
+    // ... or the candidates: rows whose key does not exceed tau[q] go to list[q][cap] in any order, cnt[q] counts them
+    const uint32_t *tau;
+    uint32_t *cnt;
+    uint64_t *list;
+    uint32_t cap;
+    const uint32_t *redo;    // nullptr, or the counts: only queries that have more than `cap` are wanted
 };
+
+// The i-th sampled tile: one of every `stride`, at a place that varies from one to the next (no period of the rows'
+// order can hide from it).
+__device__ __forceinline__ uint64_t int4_sampled(uint64_t i, uint32_t stride) {
+    uint32_t x = (uint32_t)i * 2654435761u;
+    x ^= x >> 15;
+    x *= 2246822519u;
+    x ^= x >> 13;
+    return i * stride + (uint32_t)(((uint64_t)x * stride) >> 32);
+}
 
 // Distances. A wave takes T tiles of 16 rows against QT quartets of queries; codes are the B operand (a lane has one
 // row), digits the A operand, so a lane receives the four digits of one (row, query) pair and puts them together itself.
@@ -395,12 +429,15 @@ struct Int4DistArgs {
 // the end repeat the last one against zero digits.
 // Few queries: bound by the codes' read. Many: by the six vector instructions that a group's products cost per pair
 // (two integer, two conversions, an f32 and an f64 fma; about 27 cycles against 16 of the matrix instruction).
+// NT: codes that no cache holds until the next call are read without a claim to one (4 GiB: 6.3 -> 7.2 TB/s).
 // Blocks of the same rows and different queries are neighbours on one XCD, so that the rows' codes come from its L2.
-template <int G, int QT, int T, int P, bool FUSED, class TQ>
-__global__ void __launch_bounds__(256, 2) // two waves per SIMD: at most 256 registers, so products land in vector registers, not accumulators
+template <int G, int QT, int T, int P, bool FUSED, bool NT, class TQ>
+__global__ void __launch_bounds__(int4_block(QT), QT == 3 || QT == 4 ? 4 : 2) // at most 256 registers: products land in vector registers, not accumulators
 int4_distance_kernel(Int4DistArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t s_dig[];
     Int4Query *s_info = reinterpret_cast<Int4Query *>(s_dig + (size_t)a.ku * QT * 1024);
+    constexpr uint32_t NW = int4_block(QT) / 64;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
     uint32_t x = blockIdx.x, y = 0;
     if (a.ys > 1) {
@@ -408,10 +445,18 @@ int4_distance_kernel(Int4DistArgs a) {
         y = j % a.ys;
         x = (j / a.ys) * 8 + (blockIdx.x & 7);
     }
-    const uint64_t tiles = (a.n + 15) / 16, groups = (tiles + 4 * T - 1) / (4 * T);
+    const uint64_t tiles = (a.n + 15) / 16, groups = (a.stiles + NW * T - 1) / (NW * T);
+    uint32_t *s_tau = reinterpret_cast<uint32_t *>(s_info + QT * 4);
+    if (a.redo) { // uniform over the block
+        bool any = false;
+        for (uint32_t q = y * QT * 4; q < min((y + 1) * QT * 4, a.nq); ++q) any |= a.redo[q] > a.cap;
+        if (!any) return;
+    }
+    if (a.tau && tid < QT * 4) s_tau[tid] = a.tau[min(y * QT * 4 + tid, a.nq - 1)];
+    const uint64_t out_at = h * a.dstride + r;
     auto load_digits = [&](uint32_t u0) { // digits of units [u0, u0 + ku): [unit][quartet][1 KB]
         const uint32_t cnt = min(a.ku, a.units - u0), quads = (a.nq + 3) / 4;
-        for (uint32_t i = tid; i < a.ku * QT * 64; i += 256) {
+        for (uint32_t i = tid; i < a.ku * QT * 64; i += NW * 64) {
             const uint32_t u = i / (QT * 64), q = i / 64 % QT, qq = y * QT + q;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (u < cnt && qq < quads) v = reinterpret_cast<const uint4 *>(a.dig)[((uint64_t)qq * a.units + u0 + u) * 64 + (i & 63)];
@@ -425,18 +470,39 @@ int4_distance_kernel(Int4DistArgs a) {
         if (a.units <= a.ku) load_digits(0);
     }
     __syncthreads();
+    constexpr int SC = P * 64 / G; // scales
+    struct Piece {
+        uint2 w[T][P];
+        Pack<uint16_t, SC> sc[T];
+    };
+    auto request = [&](uint64_t g, uint32_t ub, Piece &v) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) { // tile and pointers are the wave's, only the offsets are the lane's
+            const uint64_t i = (g * NW + wave) * T + t, tile = min(a.stride ? int4_sampled(i, a.stride) : i, tiles - 1);
+            const uint8_t *wp = a.codes + tile * a.units * kInt4UnitBytes;
+            const uint8_t *sp = reinterpret_cast<const uint8_t *>(a.scales + tile * 16 * a.gs);
+            const uint32_t so = min(r, (uint32_t)min(a.n - 1 - tile * 16, (uint64_t)15)) * a.gs * 2; // rows past the last: the last
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const uint8_t *at = wp + (uint64_t)min(ub + p, a.units - 1) * kInt4UnitBytes + (r * 32 + h * 8);
+                if (NT) {
+                    const uint64_t b = __builtin_nontemporal_load(reinterpret_cast<const uint64_t *>(at));
+                    v.w[t][p] = make_uint2((uint32_t)b, (uint32_t)(b >> 32));
+                } else
+                    v.w[t][p] = *reinterpret_cast<const uint2 *>(at);
+            }
+            v.sc[t] = *reinterpret_cast<const Pack<uint16_t, SC> *>(sp + 2 * (ub * 64 / G) + so); // gs is a multiple of SC: these are the row's own
+        }
+    };
+    constexpr bool AHEAD = QT >= 3; // the next piece is on its way while this one is worked on (few queries: the waves cover for each other)
+    Piece next;
+    if (AHEAD) request(min((uint64_t)x, groups - 1), 0, next);
     for (uint64_t g = x; g < groups; g += a.xs) {
-        const uint8_t *wp[T];
-        const uint16_t *sp[T];
         Int4Sum acc[T][QT];
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const uint64_t tile = min((g * 4 + (tid >> 6)) * T + t, tiles - 1);
-            wp[t] = a.codes + tile * a.units * kInt4UnitBytes + r * 32 + h * 8;
-            sp[t] = a.scales + min(tile * 16 + r, a.n - 1) * a.gs;
+        for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int q = 0; q < QT; ++q) acc[t][q] = Int4Sum{0.0, 0.f};
-        }
         for (uint32_t u0 = 0; u0 < a.units; u0 += a.ku) {
             if (!FUSED && a.units > a.ku) {
                 __syncthreads();
@@ -445,23 +511,15 @@ int4_distance_kernel(Int4DistArgs a) {
             }
             const uint32_t ue = min(u0 + a.ku, a.units);
             for (uint32_t ub = u0; ub < ue; ub += P) {
-                constexpr int SW = (P * 64 / G + 1) / 2; // words of scales
-                uint2 w[T][P];
-                ScaleWords<SW> sc[T];
-#pragma unroll
-                for (int t = 0; t < T; ++t) {
-#pragma unroll
-                    for (int p = 0; p < P; ++p) w[t][p] = *reinterpret_cast<const uint2 *>(wp[t] + (uint64_t)min(ub + p, a.units - 1) * kInt4UnitBytes);
-                    const uint32_t first = ub * 64 / G; // even: SW words from here are 4-byte aligned (P * 64 / G >= 2, or P = 2 and G = 128)
-                    if (P * 64 / G == 1)
-                        sc[t].w[0] = sp[t][first];
-                    else if (first + 2 * SW <= a.gs)
-                        sc[t] = *reinterpret_cast<const ScaleWords<SW> *>(sp[t] + first);
-                    else {
-#pragma unroll
-                        for (int i = 0; i < SW; ++i) sc[t].w[i] = *reinterpret_cast<const uint32_t *>(sp[t] + min(first + 2 * i, a.gs - 2));
-                    }
-                }
+                Piece now;
+                if (AHEAD) {
+                    now = next;
+                    const bool more = ub + P < a.units; // else the first piece of the wave's next tiles
+                    request(more ? g : min(g + a.xs, groups - 1), more ? ub + P : 0, next);
+                } else
+                    request(g, ub, now);
+                auto &w = now.w;
+                auto &sc = now.sc;
                 const i32x4_t zero = {0, 0, 0, 0};
                 constexpr uint32_t M = 0xF0F0F0F0u;
                 constexpr int PP = G == 128 ? 2 : 1; // units per group sum
@@ -480,7 +538,7 @@ int4_distance_kernel(Int4DistArgs a) {
                             const uint2 v = w[t][p0 + p];
                             b[p] = i32x4_t{(int)((v.x << 4) & M), (int)((v.y << 4) & M), (int)(v.x & M), (int)(v.y & M)};
                         }
-                        auto scale = [&](int i) { return __uint_as_float(i & 1 ? sc[t].w[i / 2] & 0xFFFF0000u : sc[t].w[i / 2] << 16); };
+                        auto scale = [&](int i) { return bf16_to_f32(sc[t].v[i]); };
                         if (G == 32) {
                             auto half = [](i32x4_t v, int i) { return (long)(uint32_t)v[2 * i] | (long)((uint64_t)(uint32_t)v[2 * i + 1] << 32); };
 #pragma unroll
@@ -505,14 +563,25 @@ int4_distance_kernel(Int4DistArgs a) {
         }
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const uint64_t row = ((g * 4 + (tid >> 6)) * T + t) * 16 + r;
-            if (row >= a.n) continue;
-            const double xsq = a.metric == kMetricDot ? 0.0 : a.sqnorm[row];
+            const uint64_t i = (g * NW + wave) * T + t, row = (a.stride ? int4_sampled(i, a.stride) : i) * 16 + r;
+            if (i >= a.stiles || (row >= a.n && !a.stride)) continue;
+            const double xsq = a.metric == kMetricDot ? 0.0 : a.sqnorm[min(row, a.n - 1)];
 #pragma unroll
             for (int q = 0; q < QT; ++q) {
-                const uint32_t qi = (y * QT + q) * 4 + h;
+                const uint32_t q0 = (y * QT + q) * 4;
                 const Int4Query qv = s_info[q * 4 + h];
-                if (qi < a.nq) a.dist[qi * a.dstride + row] = int4_finish(a.metric, acc[t][q].value() * qv.scale, xsq, qv.sq);
+                if (q0 + h >= a.nq) continue;
+                const float d = int4_finish(a.metric, acc[t][q].value(), qv.scale, xsq, qv.sq);
+                if (a.tau) {
+                    const uint32_t key = f32_key(d);
+                    if (key <= s_tau[q * 4 + h]) {
+                        const uint32_t at = atomicAdd(&a.cnt[q0 + h], 1u);
+                        if (at < a.cap) a.list[(uint64_t)(q0 + h) * a.cap + at] = (uint64_t)key << 32 | (uint32_t)row;
+                    }
+                } else {
+                    float *o = a.dist + q0 * a.dstride + i * 16;
+                    o[out_at] = row < a.n ? d : __builtin_nanf(""); // sorts last: never makes the bound smaller
+                }
             }
         }
     }
@@ -524,94 +593,184 @@ int4_distance_kernel(Int4DistArgs a) {
 // A selection is a list of (key << 32 | row) in row order; keys are f32_key (NaN after everything). A level cuts a
 // query's items into chunks and keeps each chunk's k smallest keys, equal keys by position; chunks are in row order and
 // only the last can be short of k, so positions stay the order of the rows and the padding (~0) stays at the end.
+// Many rows and queries: the distances are not written at all. The k-th smallest key of a sample of the rows bounds the
+// k-th smallest of all, a pass over the rows collects those within the bound (a few thousand), and the k smallest of the
+// collection are the answer. Where the collection overflows, the levels answer instead.
 constexpr uint32_t kTopChunk = 8192;
 constexpr uint32_t kTopMaxK = 1024;
+constexpr uint32_t kTopThreads = 512;
 
-// The k-th smallest (k >= 1) of the C >= k keys in LDS, by 8 bits at a time, and how many items with that key belong
-// to the k smallest. hist: 256 words + 2 of LDS. All threads of the block.
-__device__ __forceinline__ void block_kth_key(const uint32_t *keys, uint32_t C, uint32_t k, uint32_t *hist, uint32_t &T, uint32_t &budget) {
-    uint32_t prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (uint32_t i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0;
+struct TopkLds {
+    uint32_t hist[256];
+    uint32_t lo[kTopThreads / 64], hi[kTopThreads / 64];
+    uint32_t bin, rest;
+    uint32_t wtmp[2 * kTopThreads / 64];
+};
+
+// The k-th smallest (1 <= k <= C) of the keys key(0) .. key(C - 1), and how many of those equal to it belong to the k
+// smallest. 8 bits at a time from the highest bit in which the keys differ: distances share their leading bits, and a
+// histogram of those would be one counter that every thread adds to. All threads of a block of kTopThreads.
+template <class KeyFn>
+__device__ __forceinline__ void block_kth_key(uint32_t C, uint32_t k, KeyFn key, TopkLds &s, uint32_t &T, uint32_t &budget) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    for (uint32_t i = tid; i < C; i += kTopThreads) {
+        const uint32_t v = key(i);
+        lo = min(lo, v);
+        hi = max(hi, v);
+    }
+    lo = wave_min_u32(lo);
+    hi = ~wave_min_u32(~hi);
+    __syncthreads();
+    if ((tid & 63) == 0) {
+        s.lo[tid >> 6] = lo;
+        s.hi[tid >> 6] = hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kTopThreads / 64; ++w) {
+        lo = min(lo, s.lo[w]);
+        hi = max(hi, s.hi[w]);
+    }
+    // the bits all keys share; one 64-bit shift, no case for lo == hi: a select on it came out of the compiler wrong
+    uint32_t mask = ~(uint32_t)(0xFFFFFFFFull >> __clz((int)(lo ^ hi)));
+    uint32_t prefix = lo & mask;
+    budget = k;
+    while (mask != 0xFFFFFFFFu) {
+        const uint32_t low = 32 - __popc(mask), shift = low > 8 ? low - 8 : 0, bins = 1u << (low - shift);
+        for (uint32_t i = tid; i < 256; i += kTopThreads) s.hist[i] = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < C; i += blockDim.x)
-            if ((keys[i] & mask) == prefix) atomicAdd(&hist[(keys[i] >> shift) & 255], 1u);
+        for (uint32_t i = tid; i < C; i += kTopThreads) {
+            const uint32_t v = key(i);
+            if ((v & mask) == prefix) atomicAdd(&s.hist[(v >> shift) & (bins - 1)], 1u);
+        }
         __syncthreads();
-        if (threadIdx.x < 64) { // four bins per lane: the bin in which the running count reaches k
-            const uint32_t b = threadIdx.x * 4;
-            const uint32_t c0 = hist[b], c1 = hist[b + 1], c2 = hist[b + 2], c3 = hist[b + 3];
+        if (tid < 64) { // four bins per lane: the bin in which the running count reaches what is looked for
+            const uint32_t b = tid * 4;
+            const uint32_t c0 = s.hist[b], c1 = s.hist[b + 1], c2 = s.hist[b + 2], c3 = s.hist[b + 3];
             const uint32_t incl = wave_inclusive_sum(c0 + c1 + c2 + c3);
             uint32_t run = incl - (c0 + c1 + c2 + c3);
-            if (run < k && k <= incl) {
+            if (run < budget && budget <= incl) {
                 uint32_t bin = b;
-                if (run + c0 < k) { run += c0; ++bin;
-                    if (run + c1 < k) { run += c1; ++bin;
-                        if (run + c2 < k) { run += c2; ++bin; } } }
-                hist[256] = bin;
-                hist[257] = k - run;
+                if (run + c0 < budget) { run += c0; ++bin;
+                    if (run + c1 < budget) { run += c1; ++bin;
+                        if (run + c2 < budget) { run += c2; ++bin; } } }
+                s.bin = bin;
+                s.rest = budget - run;
             }
         }
         __syncthreads();
-        prefix |= hist[256] << shift;
-        mask |= 255u << shift;
-        k = hist[257];
+        prefix |= s.bin << shift;
+        mask |= (bins - 1) << shift;
+        budget = s.rest;
         __syncthreads();
     }
     T = prefix;
-    budget = k;
 }
 
 // Level: from f32 distances (FIRST) or from the previous level's lists. in: [nq][in_stride]; out: [nq][parts][k].
-// grid (parts, nq), block 256, LDS kTopChunk words.
+// redo: nullptr, or only queries that count more than `cap`. grid (parts, nq), block kTopThreads.
 template <bool FIRST>
-__global__ void __launch_bounds__(256)
-int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint32_t k, uint64_t *out) {
+__global__ void __launch_bounds__(kTopThreads)
+int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint32_t k, uint64_t *out, const uint32_t *redo, uint32_t cap) {
     __shared__ uint32_t keys[kTopChunk];
-    __shared__ uint32_t hist[258];
-    __shared__ uint32_t wtmp[8];
+    __shared__ TopkLds s;
+    if (redo && redo[blockIdx.y] <= cap) return;
     const uint64_t base = (uint64_t)blockIdx.x * kTopChunk;
     const uint32_t C = (uint32_t)min((uint64_t)kTopChunk, items - base), tid = threadIdx.x;
     const float *df = static_cast<const float *>(in) + (uint64_t)blockIdx.y * in_stride + base;
     const uint64_t *dl = static_cast<const uint64_t *>(in) + (uint64_t)blockIdx.y * in_stride + base;
-    for (uint32_t i = tid; i < C; i += 256) keys[i] = FIRST ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
+#pragma unroll 8
+    for (uint32_t i = tid; i < C; i += kTopThreads) keys[i] = FIRST ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
     __syncthreads();
     uint64_t *o = out + ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * k;
     uint32_t T = 0xFFFFFFFFu, budget = C;
-    if (C > k) block_kth_key(keys, C, k, hist, T, budget);
+    if (C > k) block_kth_key(C, k, [&](uint32_t i) { return keys[i]; }, s, T, budget);
     ordered_threshold_compact(
         C, T, budget, [&](uint32_t i) -> uint32_t { return keys[i]; },
-        [&](uint32_t i, uint32_t kv, uint32_t rank) { o[rank] = FIRST ? ((uint64_t)kv << 32 | (uint32_t)(base + i)) : dl[i]; }, wtmp);
-    for (uint32_t i = C + tid; i < k; i += 256) o[i] = ~0ull;
+        [&](uint32_t i, uint32_t kv, uint32_t rank) { o[rank] = FIRST ? ((uint64_t)kv << 32 | (uint32_t)(base + i)) : dl[i]; }, s.wtmp);
+    for (uint32_t i = C + tid; i < k; i += kTopThreads) o[i] = ~0ull;
 }
 
-// Last level: at most kTopChunk items; the k smallest, in order, as ids and distances.
-template <bool FIRST>
-__global__ void __launch_bounds__(256)
-int4_topk_final_kernel(const void *in, uint64_t in_stride, uint32_t items, uint32_t k, uint32_t found, const float *dist, uint64_t dstride, uint64_t *ids,
-                       float *out, uint32_t *count) {
+// The bound of a query: the k-th smallest key of its sample, and its candidate count set to zero. One block per query.
+__global__ void __launch_bounds__(kTopThreads)
+int4_topk_bound_kernel(const float *dist, uint64_t dstride, uint32_t items, uint32_t k, uint32_t *tau, uint32_t *cnt) {
+    __shared__ uint32_t keys[kTopChunk];
+    __shared__ TopkLds s;
+    const float *df = dist + (uint64_t)blockIdx.x * dstride;
+    uint32_t T, budget;
+    if (items <= kTopChunk) {
+#pragma unroll 8
+        for (uint32_t i = threadIdx.x; i < items; i += kTopThreads) keys[i] = f32_key(df[i]);
+        __syncthreads();
+        block_kth_key(items, k, [&](uint32_t i) { return keys[i]; }, s, T, budget);
+    } else
+        block_kth_key(items, k, [&](uint32_t i) { return f32_key(df[i]); }, s, T, budget);
+    if (threadIdx.x == 0) {
+        tau[blockIdx.x] = T;
+        cnt[blockIdx.x] = 0;
+    }
+}
+
+__device__ __forceinline__ float f32_of_key(uint32_t k) { // NaN for the NaN's key; the two zeros are one
+    if (k == 0xFFFFFFFFu) return __builtin_nanf("");
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+// Last level: at most kTopChunk items; the k smallest, in order, as ids and distances. KIND 0: distances in row order,
+// 1: a level's list, 2: a collection in any order, count[q] of them (left alone where they overflowed).
+template <int KIND>
+__global__ void __launch_bounds__(kTopThreads)
+int4_topk_final_kernel(const void *in, uint64_t in_stride, uint32_t items, uint32_t k, uint32_t found, const uint32_t *cnt, uint32_t cap, uint64_t *ids, float *out,
+                       uint32_t *count) {
     __shared__ uint32_t keys[kTopChunk];
     __shared__ uint64_t sel[kTopMaxK];
-    __shared__ uint32_t hist[258];
-    __shared__ uint32_t wtmp[8];
+    __shared__ TopkLds s;
+    __shared__ uint32_t s_n;
     const uint32_t tid = threadIdx.x, q = blockIdx.x;
+    if (KIND == 2) {
+        items = cnt[q];
+        if (items > cap) return;
+    } else if (cnt && cnt[q] <= cap)
+        return;
     const float *df = static_cast<const float *>(in) + (uint64_t)q * in_stride;
     const uint64_t *dl = static_cast<const uint64_t *>(in) + (uint64_t)q * in_stride;
-    for (uint32_t i = tid; i < items; i += 256) keys[i] = FIRST ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
+#pragma unroll 8
+    for (uint32_t i = tid; i < items; i += kTopThreads) keys[i] = KIND == 0 ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
     const uint32_t width = next_pow2(min(k, items));
-    for (uint32_t i = tid; i < width; i += 256) sel[i] = ~0ull;
+    for (uint32_t i = tid; i < width; i += kTopThreads) sel[i] = ~0ull;
+    if (tid == 0) s_n = 0;
     __syncthreads();
     uint32_t T = 0xFFFFFFFFu, budget = items;
-    if (items > k) block_kth_key(keys, items, k, hist, T, budget);
-    ordered_threshold_compact(
-        items, T, budget, [&](uint32_t i) -> uint32_t { return keys[i]; },
-        [&](uint32_t i, uint32_t kv, uint32_t rank) { sel[rank] = FIRST ? ((uint64_t)kv << 32 | i) : dl[i]; }, wtmp);
+    if (items > k) block_kth_key(items, k, [&](uint32_t i) { return keys[i]; }, s, T, budget);
+    if (KIND == 2) {
+        // of the candidates equal to the k-th key the `budget` lowest rows: the budget-th smallest row among them
+        uint32_t R = 0xFFFFFFFFu, rest;
+        if (items > k) {
+            uint32_t ties = 0;
+            for (uint32_t i = tid; i < items; i += kTopThreads) ties += keys[i] == T ? 1u : 0u;
+            if (ties) atomicAdd(&s_n, ties);
+            __syncthreads();
+            ties = s_n;
+            __syncthreads();
+            if (tid == 0) s_n = 0;
+            if (ties > budget) block_kth_key(items, budget, [&](uint32_t i) { return keys[i] == T ? (uint32_t)dl[i] : 0xFFFFFFFFu; }, s, R, rest);
+            __syncthreads();
+        }
+        for (uint32_t i = tid; i < items; i += kTopThreads) {
+            const uint64_t v = keys[i] <= T ? dl[i] : ~0ull;
+            if (keys[i] < T || (keys[i] == T && (uint32_t)v <= R)) sel[atomicAdd(&s_n, 1u)] = v;
+        }
+    } else
+        ordered_threshold_compact(
+            items, T, budget, [&](uint32_t i) -> uint32_t { return keys[i]; },
+            [&](uint32_t i, uint32_t kv, uint32_t rank) { sel[rank] = KIND == 0 ? ((uint64_t)kv << 32 | i) : dl[i]; }, s.wtmp);
     __syncthreads();
     block_sort_u64(sel, width);
-    for (uint32_t i = tid; i < k; i += 256) {
+    for (uint32_t i = tid; i < k; i += kTopThreads) {
         const bool have = i < found;
-        const uint32_t row = have ? (uint32_t)sel[i] : 0u;
-        ids[(uint64_t)q * k + i] = have ? (uint64_t)row : ~0ull;
-        out[(uint64_t)q * k + i] = have ? dist[(uint64_t)q * dstride + row] : __builtin_huge_valf();
+        ids[(uint64_t)q * k + i] = have ? (uint64_t)(uint32_t)sel[i] : ~0ull;
+        out[(uint64_t)q * k + i] = have ? f32_of_key((uint32_t)(sel[i] >> 32)) : __builtin_huge_valf();
     }
     if (count && tid == 0) count[q] = found;
 }

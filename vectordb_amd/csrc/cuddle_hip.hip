@@ -2998,8 +2998,10 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
             w.sel[0] = take((size_t)qc * parts * k * 8);
             w.sel[1] = take((size_t)qc * ((parts * k + kTopChunk - 1) / kTopChunk) * k * 8);
         }
-        // a sample of 4096 rows, or as many as leave half of the collection's room expected to be filled
-        const uint64_t want = std::max<uint64_t>(256, (k * n / (kTopChunk / 2) + 15) / 16);
+        // k of a sample of S rows bound k n / S of all: enough to expect 512 candidates, at most a sixteenth of the
+        // rows, but no fewer than expect half of the collection's room to be filled
+        const uint64_t kn = (uint64_t)k * n;
+        const uint64_t rows = std::max<uint64_t>({4096, std::min<uint64_t>(kn / 512, n / 16), kn / (kTopChunk / 2)}), want = (rows + 15) / 16;
         if (qc * n >= kInt4SampleFrom && tiles / want >= 8) {
             w.stride = (uint32_t)(tiles / want);
             w.stiles = tiles / w.stride;
@@ -3015,7 +3017,7 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
 // Launch shapes of the distance kernel. One quartet of queries: codes are the bound, so many of them are requested at a
 // time (16 pieces of 512 bytes per wave). More: QT quartets per wave, the count among those built that costs least,
 // pairs of (row, query) at about 27 cycles and the unpacking of the codes, once per QT, at about as much.
-constexpr uint32_t int4_lds_kb(int qt) { return qt >= 3 ? 150u : 64u; } // digits per block: one block of 8 waves per CU, or two of 4 and more
+constexpr uint32_t int4_lds_kb(int qt) { return qt >= 3 ? 144u : 64u; } // digits per block: one block of 8 waves per CU, or two of 4 and more
 
 template <int G, int QT, int T, int P, bool FUSED, bool NT, class TQ>
 void int4_launch(Int4DistArgs a, hipStream_t s) {
@@ -3023,14 +3025,16 @@ void int4_launch(Int4DistArgs a, hipStream_t s) {
     a.ku = std::min<uint32_t>((a.units + P - 1) / P * P, int4_lds_kb(QT) / QT / P * P);
     a.ys = ((a.nq + 3) / 4 + QT - 1) / QT;
     const uint64_t groups = (a.stiles + NW * T - 1) / (NW * T);
-    const size_t lds = (size_t)a.ku * QT * 1024 + QT * 4 * (sizeof(Int4Query) + 4);
+    constexpr size_t extra = QT * 4 * (sizeof(Int4Query) + 4 + sizeof(Int4Test)) + NW * 128 * sizeof(Int4Held); // candidates held back by the search's pass
+    static_assert(int4_lds_kb(QT) * 1024 + extra <= 160u << 10, "LDS");
+    const size_t lds = (size_t)a.ku * QT * 1024 + QT * 4 * (sizeof(Int4Query) + 4 + sizeof(Int4Test)) + (a.tau ? NW * 128 * sizeof(Int4Held) : 0);
     static_assert(P * 64 % G == 0, "whole groups");
     const void *kernel = (const void *)int4_distance_kernel<G, QT, T, P, FUSED, NT, TQ>;
     static std::once_flag once[kMaxDevices]; // more than 64 KB of LDS: the kernel's limit is raised, once per device
     int dev = 0;
     (void)hipGetDevice(&dev);
     std::call_once(once[dev & (kMaxDevices - 1)], [kernel] {
-        (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(int4_lds_kb(QT) * 1024 + QT * 4 * (sizeof(Int4Query) + 4)));
+        (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(int4_lds_kb(QT) * 1024 + extra));
     });
     // As many blocks as the chip holds at a time, each walking over the rows: blocks per CU of this kernel and LDS size
     static std::atomic<uint64_t> known{0}; // (lds << 32 | blocks), what the last call asked about
@@ -3069,9 +3073,9 @@ void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStre
         return;
     }
     uint32_t best = 1, cost = ~0u;
-    static const char *force = getenv("CUDDLE_QT");
     for (uint32_t qt : {1u, 2u, 3u, 4u, 6u, 8u}) {
-        if (force && (uint32_t)atoi(force) != qt) continue;
+        if (qt > 4 && a.units < 6) break; // short rows: the finish weighs as much as the products, and four waves per SIMD
+                                          // (QT <= 4) hide more of it than two (1M x 128, 100 queries: 167 us against 206)
         const uint32_t ys = (quads + qt - 1) / qt;
         const bool whole = a.units <= int4_lds_kb((int)qt) / qt; // else the digits are fetched anew for every 256 rows: about as much again
         const uint32_t c = ys * (qt * (whole ? 1 : 2) + 1);
@@ -3086,7 +3090,10 @@ void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStre
     case 3: int4_launch<G, 3, 2, 2, false, false, float>(a, s); break;
     case 4: int4_launch<G, 4, 2, 2, false, false, float>(a, s); break;
     case 6: int4_launch<G, 6, 2, 2, false, false, float>(a, s); break;
-    default: int4_launch<G, 8, 2, 2, false, false, float>(a, s); break;
+    default:
+        if (a.units >= 4) int4_launch<G, 8, 2, 4, false, false, float>(a, s);
+        else int4_launch<G, 8, 2, 2, false, false, float>(a, s);
+        break;
     }
 }
 
@@ -3271,7 +3278,12 @@ extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows,
             a.stride = w.stride;
             a.stiles = w.stiles;
             int4_run(a, rows->group, type, fused, s);
-            hipLaunchKernelGGL(int4_topk_bound_kernel, dim3(nq), dim3(kTopThreads), 0, s, dist, a.dstride, (uint32_t)(w.stiles * 16), k, tau, cnt);
+            const uint32_t items = (uint32_t)(w.stiles * 16), in_lds = items <= (36u << 10) ? 1u : 0u;
+            static std::once_flag once[kMaxDevices];
+            std::call_once(once[device_id & (kMaxDevices - 1)], [] {
+                (void)hipFuncSetAttribute((const void *)int4_topk_bound_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 36 << 12);
+            });
+            hipLaunchKernelGGL(int4_topk_bound_kernel, dim3(nq), dim3(kTopThreads), in_lds ? items * 4 : 0, s, dist, a.dstride, items, k, in_lds, tau, cnt);
             a = all;
             a.tau = tau;
             a.cnt = cnt;

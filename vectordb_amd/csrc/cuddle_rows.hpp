@@ -412,6 +412,45 @@ struct Int4DistArgs {
     const uint32_t *redo;    // nullptr, or the counts: only queries that have more than `cap` are wanted
 };
 
+struct Int4Held { uint32_t key, row, q; };
+
+// The candidates' pass asks of nearly every (row, query) pair only whether its distance is beyond the bound, and f32
+// answers that where it is not close. With S = the sum rounded to f32 a distance is t = A * S * R + B plus a constant of
+// the query: l2 A = -2 scale, B = |x|^2; dot A = -scale; cosine A = -scale / |q|, R = 1 / |x|. S is off by at most 2^-23
+// of itself and of its upper part, which differ by less than 2^-6 |x||q| / scale (the lower digits are at most 2^-13 of
+// the largest component, times sqrt(dim)). |S| scale <= |x||q|, at most (|x|^2 + |q|^2) / 2: for l2 all roundings together
+// stay below 2^-20 (|x|^2 + |q|^2), for cosine below 2^-20, taken off B and added to C = bound - constant beforehand.
+// dot has no such measure at hand: S is moved by 2^-20 of itself and its lower part. t > C: surely beyond. What is not a
+// number, or too large or small for f32, is not "beyond" and goes on to the exact evaluation.
+struct Int4Test {
+    float A, C;
+};
+__device__ __forceinline__ Int4Test int4_test(uint32_t metric, uint32_t tau, const Int4Query &q) {
+    constexpr double up = 1.0 / (1 << 19);
+    const Int4Test all{0.f, __builtin_huge_valf()}; // every pair goes on
+    if (tau >= 0xFF800000u) return all; // bound +inf or NaN
+    const double t = (double)__uint_as_float(tau & 0x80000000u ? tau & 0x7FFFFFFFu : ~tau);
+    const double A = metric == kMetricDot ? -q.scale : metric == kMetricCosine ? -q.scale / sqrt(q.sq) : -2.0 * q.scale;
+    const double c = metric == kMetricDot ? 0.0 : metric == kMetricCosine ? 1.0 : q.sq, mag = fabs(t) + c;
+    if (!(fabs(A) > 1e-30 && fabs(A) < 1e30 && mag < 1e30)) return all;
+    return Int4Test{(float)A, (float)(t - c + up * mag)};
+}
+// Row side: B lowered, R; NaN beyond f32's range.
+__device__ __forceinline__ float int4_test_row(uint32_t metric, double xsq) {
+    if (metric == kMetricDot) return 0.f;
+    if (!(xsq < 1e30 && xsq > 1e-30)) return __builtin_nanf("");
+    return metric == kMetricCosine ? (float)(1.0 / sqrt(xsq)) : (float)(xsq * (1.0 - 1.0 / (1 << 19)));
+}
+template <uint32_t METRIC>
+__device__ __forceinline__ bool int4_beyond(double hi, float lo, const Int4Test &q, float row) {
+    float S = __builtin_fmaf((float)hi, 65536.f, lo);
+    if (METRIC == kMetricL2) return __builtin_fmaf(q.A, S, row) > q.C;
+    if (METRIC == kMetricCosine) return q.A * (S * row) > q.C;
+    S = __builtin_fmaf(fabsf(lo) + fabsf(S), 0x1p-20f, S); // A < 0: a larger S is a smaller t
+    const float t = q.A * S;
+    return t > q.C && t < 3.0e38f;
+}
+
 // The i-th sampled tile: one of every `stride`, at a place that varies from one to the next (no period of the rows'
 // order can hide from it).
 __device__ __forceinline__ uint64_t int4_sampled(uint64_t i, uint32_t stride) {
@@ -447,12 +486,43 @@ int4_distance_kernel(Int4DistArgs a) {
     }
     const uint64_t tiles = (a.n + 15) / 16, groups = (a.stiles + NW * T - 1) / (NW * T);
     uint32_t *s_tau = reinterpret_cast<uint32_t *>(s_info + QT * 4);
+    Int4Test *s_test = reinterpret_cast<Int4Test *>(s_tau + QT * 4);
     if (a.redo) { // uniform over the block
         bool any = false;
         for (uint32_t q = y * QT * 4; q < min((y + 1) * QT * 4, a.nq); ++q) any |= a.redo[q] > a.cap;
         if (!any) return;
     }
     if (a.tau && tid < QT * 4) s_tau[tid] = a.tau[min(y * QT * 4 + tid, a.nq - 1)];
+    // Candidates wait in LDS, the wave's own 128 places, and go out 64 at a time: one trip to the counters for 64 of them
+    // instead of one for each.
+    Int4Held *s_held = reinterpret_cast<Int4Held *>(s_test + QT * 4) + wave * 128;
+    uint32_t held = 0;
+    auto wave_sync = []() {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    auto flush = [&](uint32_t count) { // the first `count` <= 64
+        if (lane < count) {
+            const Int4Held c = s_held[lane];
+            const uint32_t at = atomicAdd(&a.cnt[c.q], 1u);
+            if (at < a.cap) a.list[(uint64_t)c.q * a.cap + at] = (uint64_t)c.key << 32 | c.row;
+        }
+    };
+    auto keep = [&](bool take, uint32_t key, uint32_t row, uint32_t q) { // all lanes of the wave call
+        const uint64_t m = __ballot(take);
+        if (!m) return;
+        if (take) s_held[held + (uint32_t)__popcll(m & lanemask_lt())] = Int4Held{key, row, q};
+        held += (uint32_t)__popcll(m);
+        wave_sync();
+        if (held >= 64) {
+            flush(64);
+            wave_sync();
+            held -= 64;
+            if (lane < held) s_held[lane] = s_held[64 + lane];
+            wave_sync();
+        }
+    };
     const uint64_t out_at = h * a.dstride + r;
     auto load_digits = [&](uint32_t u0) { // digits of units [u0, u0 + ku): [unit][quartet][1 KB]
         const uint32_t cnt = min(a.ku, a.units - u0), quads = (a.nq + 3) / 4;
@@ -470,6 +540,11 @@ int4_distance_kernel(Int4DistArgs a) {
         if (a.units <= a.ku) load_digits(0);
     }
     __syncthreads();
+    if (a.tau) {
+        if (tid < QT * 4) // places past the last query: nothing passes
+            s_test[tid] = y * QT * 4 + tid < a.nq ? int4_test(a.metric, s_tau[tid], s_info[tid]) : Int4Test{0.f, -__builtin_huge_valf()};
+        __syncthreads();
+    }
     constexpr int SC = P * 64 / G; // scales
     struct Piece {
         uint2 w[T][P];
@@ -498,6 +573,14 @@ int4_distance_kernel(Int4DistArgs a) {
     Piece next;
     if (AHEAD) request(min((uint64_t)x, groups - 1), 0, next);
     for (uint64_t g = x; g < groups; g += a.xs) {
+        uint64_t row[T];
+        double xsq[T]; // on its way from here, needed after the last piece
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const uint64_t i = (g * NW + wave) * T + t;
+            row[t] = (a.stride ? int4_sampled(i, a.stride) : i) * 16 + r;
+            xsq[t] = a.metric == kMetricDot ? 0.0 : a.sqnorm[min(row[t], a.n - 1)];
+        }
         Int4Sum acc[T][QT];
 #pragma unroll
         for (int t = 0; t < T; ++t)
@@ -516,6 +599,7 @@ int4_distance_kernel(Int4DistArgs a) {
                     now = next;
                     const bool more = ub + P < a.units; // else the first piece of the wave's next tiles
                     request(more ? g : min(g + a.xs, groups - 1), more ? ub + P : 0, next);
+                    __builtin_amdgcn_sched_barrier(0); // all of it now, not next to its use
                 } else
                     request(g, ub, now);
                 auto &w = now.w;
@@ -563,28 +647,43 @@ int4_distance_kernel(Int4DistArgs a) {
         }
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const uint64_t i = (g * NW + wave) * T + t, row = (a.stride ? int4_sampled(i, a.stride) : i) * 16 + r;
-            if (i >= a.stiles || (row >= a.n && !a.stride)) continue;
-            const double xsq = a.metric == kMetricDot ? 0.0 : a.sqnorm[min(row, a.n - 1)];
+            const uint64_t i = (g * NW + wave) * T + t;
+            if (a.tau) {
+                const float rt = int4_test_row(a.metric, xsq[t]);
+                const bool real = i < a.stiles && row[t] < a.n;
+                auto pass = [&](auto metric) {
+                    constexpr uint32_t M = decltype(metric)::value;
+                    uint64_t any = 0;
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) any |= __ballot(!int4_beyond<M>(acc[t][q].hi, acc[t][q].lo, s_test[q * 4 + h], rt));
+                    if (!any) return;
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) {
+                        const bool take = real && !int4_beyond<M>(acc[t][q].hi, acc[t][q].lo, s_test[q * 4 + h], rt);
+                        if (!__ballot(take)) continue;
+                        const uint32_t qi = (y * QT + q) * 4 + h;
+                        const Int4Query qv = s_info[q * 4 + h];
+                        const uint32_t key = f32_key(int4_finish(M, acc[t][q].value(), qv.scale, xsq[t], qv.sq));
+                        keep(take && qi < a.nq && key <= s_tau[q * 4 + h], key, (uint32_t)row[t], qi);
+                    }
+                };
+                if (a.metric == kMetricL2) pass(std::integral_constant<uint32_t, kMetricL2>{});
+                else if (a.metric == kMetricCosine) pass(std::integral_constant<uint32_t, kMetricCosine>{});
+                else pass(std::integral_constant<uint32_t, kMetricDot>{});
+                continue;
+            }
+            if (i >= a.stiles || (row[t] >= a.n && !a.stride)) continue;
 #pragma unroll
             for (int q = 0; q < QT; ++q) {
                 const uint32_t q0 = (y * QT + q) * 4;
                 const Int4Query qv = s_info[q * 4 + h];
-                if (q0 + h >= a.nq) continue;
-                const float d = int4_finish(a.metric, acc[t][q].value(), qv.scale, xsq, qv.sq);
-                if (a.tau) {
-                    const uint32_t key = f32_key(d);
-                    if (key <= s_tau[q * 4 + h]) {
-                        const uint32_t at = atomicAdd(&a.cnt[q0 + h], 1u);
-                        if (at < a.cap) a.list[(uint64_t)(q0 + h) * a.cap + at] = (uint64_t)key << 32 | (uint32_t)row;
-                    }
-                } else {
-                    float *o = a.dist + q0 * a.dstride + i * 16;
-                    o[out_at] = row < a.n ? d : __builtin_nanf(""); // sorts last: never makes the bound smaller
-                }
+                float *o = a.dist + q0 * a.dstride + i * 16;
+                const float d = int4_finish(a.metric, acc[t][q].value(), qv.scale, xsq[t], qv.sq);
+                if (q0 + h < a.nq) o[out_at] = row[t] < a.n ? d : __builtin_nanf(""); // NaN sorts last: never makes the bound smaller
             }
         }
     }
+    if (a.tau) flush(held);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -692,18 +791,19 @@ int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint3
     for (uint32_t i = C + tid; i < k; i += kTopThreads) o[i] = ~0ull;
 }
 
-// The bound of a query: the k-th smallest key of its sample, and its candidate count set to zero. One block per query.
+// The bound of a query: the k-th smallest key of its sample, and its candidate count set to zero. One block per query;
+// the keys in LDS where they fit (items words of dynamic LDS, or none).
 __global__ void __launch_bounds__(kTopThreads)
-int4_topk_bound_kernel(const float *dist, uint64_t dstride, uint32_t items, uint32_t k, uint32_t *tau, uint32_t *cnt) {
-    __shared__ uint32_t keys[kTopChunk];
+int4_topk_bound_kernel(const float *dist, uint64_t dstride, uint32_t items, uint32_t k, uint32_t in_lds, uint32_t *tau, uint32_t *cnt) {
+    extern __shared__ uint32_t s_keys[];
     __shared__ TopkLds s;
     const float *df = dist + (uint64_t)blockIdx.x * dstride;
     uint32_t T, budget;
-    if (items <= kTopChunk) {
+    if (in_lds) {
 #pragma unroll 8
-        for (uint32_t i = threadIdx.x; i < items; i += kTopThreads) keys[i] = f32_key(df[i]);
+        for (uint32_t i = threadIdx.x; i < items; i += kTopThreads) s_keys[i] = f32_key(df[i]);
         __syncthreads();
-        block_kth_key(items, k, [&](uint32_t i) { return keys[i]; }, s, T, budget);
+        block_kth_key(items, k, [&](uint32_t i) { return s_keys[i]; }, s, T, budget);
     } else
         block_kth_key(items, k, [&](uint32_t i) { return f32_key(df[i]); }, s, T, budget);
     if (threadIdx.x == 0) {

@@ -2921,6 +2921,22 @@ struct DeviceGuard { // the calls below leave the caller's current device as it 
 };
 
 unsigned grid_for(uint64_t blocks) { return (unsigned)std::min<uint64_t>(std::max<uint64_t>(blocks, 1), 1u << 20); }
+// Shape of the lookups: a row's pieces over at most 256 threads (grid.y parts of them), several rows per block where
+// they fit, four per thread where there are enough rows to fill the chip that way (four neighbouring 4-bit rows are the
+// same 128-byte lines: decoding 1M x 960 to f32 takes 829 us, 1196 with one row per block, 1036 with sixteen).
+struct RowShape {
+    uint32_t w, rpi, rpb;
+    dim3 grid;
+};
+RowShape row_shape(uint32_t pieces, uint64_t rows) {
+    RowShape r;
+    const uint32_t parts = (pieces + 255) / 256;
+    r.w = (pieces + parts - 1) / parts;
+    r.rpi = 256 / r.w;
+    r.rpb = rows * parts / r.rpi > 4096 ? r.rpi * 4 : r.rpi;
+    r.grid = dim3(grid_for((rows + r.rpb - 1) / r.rpb), parts);
+    return r;
+}
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 uint32_t type_size(uint32_t type) { return type == CUDDLE_TYPE_F32 ? 4u : 2u; }
 cuddle_status check_type(uint32_t type) { return type > CUDDLE_TYPE_BF16 ? fail(CUDDLE_ERR_BAD_ARG, "unknown element type %u", type) : CUDDLE_OK; }
@@ -3056,6 +3072,10 @@ void int4_launch(Int4DistArgs a, hipStream_t s) {
     hipLaunchKernelGGL((int4_distance_kernel<G, QT, T, P, FUSED, NT, TQ>), dim3((unsigned)(a.xs * a.ys)), dim3(int4_block(QT)), lds, s, a);
 }
 
+#ifndef QT_T
+#define QT_T 2
+#define QT_P 4
+#endif
 template <int G>
 void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStream_t s) {
     const uint32_t quads = (a.nq + 3) / 4;
@@ -3067,8 +3087,8 @@ void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStre
             const bool nt = (a.n + 15) / 16 * a.units * kInt4UnitBytes > (256ull << 20) && !a.stride;
             if (few_units && nt) int4_launch<G, 1, 4, 2, true, true, TQ>(a, s);
             else if (few_units) int4_launch<G, 1, 4, 2, true, false, TQ>(a, s);
-            else if (nt) int4_launch<G, 1, 2, G == 32 ? 4 : 8, true, true, TQ>(a, s);
-            else int4_launch<G, 1, 2, G == 32 ? 4 : 8, true, false, TQ>(a, s);
+            else if (nt) int4_launch<G, 1, QT_T, QT_P, true, true, TQ>(a, s);
+            else int4_launch<G, 1, QT_T, QT_P, true, false, TQ>(a, s);
         });
         return;
     }
@@ -3166,16 +3186,21 @@ extern "C" cuddle_status cuddle_int4_encode_device(const cuddle_int4_rows *rows,
     DeviceGuard guard;
     ST_TRY(guard.enter(device_id));
     if (count == 0) return CUDDLE_OK;
-    const uint64_t tiles = (first_row % 16 + count + 15) / 16;
+    // few rows: a wave each, or the chip stays empty (1000 x 768: 12.4 -> 6.3 us; 1M x 960 loses 5 %)
+    const bool wide = count < 8192 && rows->dim > 128;
+    const uint32_t rpb = wide ? 4 : 16;
+    const uint64_t blocks = (first_row % rpb + count + rpb - 1) / rpb;
     const bool vec = aligned16(d_vectors) && row_stride * type_size(type) % 16 == 0;
     with_type(type, [&](auto z) {
         using T = decltype(z);
         auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(grid_for(tiles)), dim3(256), 0, (hipStream_t)stream_, (const T *)d_vectors, row_stride, first_row, count, rows->dim,
-                               rows->group, (uint8_t *)rows->codes, (uint16_t *)rows->scales, (double *)rows->sqnorm, tiles);
+            hipLaunchKernelGGL(kernel, dim3(grid_for(blocks)), dim3(256), 0, (hipStream_t)stream_, (const T *)d_vectors, row_stride, first_row, count, rows->dim,
+                               rows->group, (uint8_t *)rows->codes, (uint16_t *)rows->scales, (double *)rows->sqnorm, blocks);
         };
-        if (vec) go(int4_encode_kernel<T, true>);
-        else go(int4_encode_kernel<T, false>);
+        if (vec && wide) go(int4_encode_kernel<T, true, 64>);
+        else if (vec) go(int4_encode_kernel<T, true, 16>);
+        else if (wide) go(int4_encode_kernel<T, false, 64>);
+        else go(int4_encode_kernel<T, false, 16>);
     });
     HIP_TRY(hipGetLastError());
     return CUDDLE_OK;
@@ -3192,18 +3217,20 @@ extern "C" cuddle_status cuddle_int4_lookup_device(const cuddle_int4_rows *rows,
     DeviceGuard guard;
     ST_TRY(guard.enter(device_id));
     if (n_ids == 0) return CUDDLE_OK;
-    const uint32_t ppr = (rows->dim + 7) / 8, rpb = std::max<uint32_t>(1, 256 / ppr);
+    const RowShape sh = row_shape((rows->dim * type_size(out_type) + 15) / 16, n_ids);
     const bool vec = aligned16(d_out) && (uint64_t)rows->dim * type_size(out_type) % 16 == 0;
     with_type(out_type, [&](auto z) {
         using T = decltype(z);
         with_id(id_bits, [&](auto zi) {
             using I = decltype(zi);
             auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(grid_for((n_ids + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream_, (const uint8_t *)rows->codes,
-                                   (const uint16_t *)rows->scales, rows->n, rows->dim, rows->group, (const I *)d_ids, n_ids, scale, (T *)d_out, rpb);
+                hipLaunchKernelGGL(kernel, sh.grid, dim3(256), 0, (hipStream_t)stream_, (const uint8_t *)rows->codes, (const uint16_t *)rows->scales, rows->n,
+                                   rows->dim, rows->group, (const I *)d_ids, n_ids, scale, (T *)d_out, sh.w, sh.rpi, sh.rpb);
             };
-            if (vec) go(int4_lookup_kernel<T, I, true>);
-            else go(int4_lookup_kernel<T, I, false>);
+            if (!d_ids && vec) go(int4_lookup_kernel<T, I, true, 1>);
+            else if (!d_ids) go(int4_lookup_kernel<T, I, false, 1>);
+            else if (vec) go(int4_lookup_kernel<T, I, true, 4>);
+            else go(int4_lookup_kernel<T, I, false, 4>);
         });
     });
     HIP_TRY(hipGetLastError());
@@ -3337,14 +3364,14 @@ extern "C" cuddle_status cuddle_rows_lookup_device(const void *d_table, uint32_t
     if (n_ids == 0) return CUDDLE_OK;
     const uint32_t ts = type_size(type);
     const bool vec = aligned16(d_table) && aligned16(d_out) && row_stride * ts % 16 == 0 && (uint64_t)dim * ts % 16 == 0;
-    const uint32_t per = vec ? 16 / ts : 1, ppr = (dim + per - 1) / per, rpb = std::max<uint32_t>(1, 256 / ppr);
+    const RowShape sh = row_shape(vec ? dim / (16 / ts) : dim, n_ids);
     with_type(type, [&](auto z) {
         using T = decltype(z);
         with_id(id_bits, [&](auto zi) {
             using I = decltype(zi);
             auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(grid_for((n_ids + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream_, (const T *)d_table, row_stride, n_rows, dim,
-                                   (const I *)d_ids, n_ids, scale, (T *)d_out, rpb);
+                hipLaunchKernelGGL(kernel, sh.grid, dim3(256), 0, (hipStream_t)stream_, (const T *)d_table, row_stride, n_rows, dim, (const I *)d_ids, n_ids, scale,
+                                   (T *)d_out, sh.w, sh.rpi, sh.rpb);
             };
             if (vec) go(rows_lookup_kernel<T, I, 16 / sizeof(T)>);
             else go(rows_lookup_kernel<T, I, 1>);
@@ -3355,11 +3382,11 @@ extern "C" cuddle_status cuddle_rows_lookup_device(const void *d_table, uint32_t
 }
 
 namespace {
-// Work space of a gradient: sorted keys and places (two of each for more than one pass), tile histograms, the map of
+// Work space of a gradient: sorted (row, place) pairs (two buffers for more than one pass), tile histograms, the map of
 // named rows, the parts of runs that chunks cut.
 struct GradWs {
-    uint32_t R = 0, chunks = 0;
-    size_t key[2] = {0, 0}, pos[2] = {0, 0}, hist = 0, total = 0, named = 0, part = 0, bytes = 0;
+    uint32_t R = 0, chunks = 0, tile = 0;
+    size_t place[2] = {0, 0}, hist = 0, total = 0, named = 0, part = 0, bytes = 0;
 };
 GradWs grad_ws(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
     GradWs w;
@@ -3369,15 +3396,15 @@ GradWs grad_ws(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
         at += round_ws(b);
         return p;
     };
-    w.R = n_ids > (128u << 10) ? 32 : n_ids > kSortSmall ? 16 : 8; // enough chunks to fill the chip, few enough cut runs
+    // enough chunks to fill the chip, few enough cut runs (64K places of 768, skewed: 28 + 18 us with 16, 28 + 10 with 24;
+    // 1M places of 128: 231 + 23 with 16, 232 + 12 with 64)
+    w.R = n_ids > (128u << 10) ? 64 : n_ids > kSortSmall ? 24 : 8;
     w.chunks = (uint32_t)((n_ids + w.R - 1) / w.R);
     const bool small = n_ids <= kSortSmall;
-    for (int i = 0; i < (small ? 1 : 2); ++i) {
-        w.key[i] = take(n_ids * 4);
-        w.pos[i] = take(n_ids * 4);
-    }
+    for (int i = 0; i < (small ? 1 : 2); ++i) w.place[i] = take(n_ids * 8);
     if (!small) {
-        w.hist = take(((n_ids + kSortTile - 1) / kSortTile << kSortMaxBits) * 4);
+        w.tile = n_ids <= (256u << 10) ? 1024 : 4096;
+        w.hist = take(((n_ids + w.tile - 1) / w.tile << kSortMaxBits) * 4);
         w.total = take(4u << kSortMaxBits);
         w.named = take(n_rows);
     }
@@ -3436,34 +3463,35 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
         with_id(id_bits, [&](auto zi) {
             using I = decltype(zi);
             hipLaunchKernelGGL(rows_sort_small_kernel<I>, dim3(1 + zero_blocks), dim3(1024), 0, s, (const I *)d_ids, t, n_rows, (row_bits + 7) / 8,
-                               (uint32_t *)(ws + w.key[0]), (uint32_t *)(ws + w.pos[0]), d_grad, grad_bytes);
+                               (uint2 *)(ws + w.place[0]), d_grad, grad_bytes);
         });
     } else {
         uint32_t *hist = (uint32_t *)(ws + w.hist), *total = (uint32_t *)(ws + w.total);
-        const uint32_t tiles = (t + kSortTile - 1) / kSortTile, passes = (row_bits + kSortMaxBits - 1) / kSortMaxBits, bits = (row_bits + passes - 1) / passes;
+        const uint32_t tiles = (t + w.tile - 1) / w.tile, passes = (row_bits + kSortMaxBits - 1) / kSortMaxBits, bits = (row_bits + passes - 1) / passes;
         const unsigned clear = add ? 0 : (unsigned)std::min<uint64_t>((n_rows + 16383) / 16384, 256);
         named = add ? nullptr : ws + w.named;
-        for (uint32_t p = 0; p < passes; ++p, cur ^= 1) {
-            const uint32_t shift = p * bits;
-            uint32_t *okey = (uint32_t *)(ws + w.key[cur ^ 1]), *opos = (uint32_t *)(ws + w.pos[cur ^ 1]);
-            const uint32_t *ikey = (const uint32_t *)(ws + w.key[cur]), *ipos = (const uint32_t *)(ws + w.pos[cur]);
-            auto scan = [&]() { hipLaunchKernelGGL(rows_sort_scan_kernel, dim3(((1u << bits) + 63) / 64), dim3(1024), 0, s, hist, tiles, 1u << bits, total); };
-            if (p == 0)
-                with_id(id_bits, [&](auto zi) {
-                    using I = decltype(zi);
-                    hipLaunchKernelGGL((rows_sort_hist_kernel<true, I>), dim3(tiles + clear), dim3(256), 0, s, d_ids, t, n_rows, shift, bits, tiles, hist, ws + w.named);
-                    scan();
-                    hipLaunchKernelGGL((rows_sort_scatter_kernel<true, I>), dim3(tiles), dim3(256), 0, s, d_ids, (const uint32_t *)nullptr, t, n_rows, shift, bits, hist,
-                                       total, okey, opos, named);
-                });
-            else {
-                hipLaunchKernelGGL((rows_sort_hist_kernel<false, int32_t>), dim3(tiles), dim3(256), 0, s, (const void *)ikey, t, n_rows, shift, bits, tiles, hist,
-                                   (uint8_t *)nullptr);
-                scan();
-                hipLaunchKernelGGL((rows_sort_scatter_kernel<false, int32_t>), dim3(tiles), dim3(256), 0, s, (const void *)ikey, ipos, t, n_rows, shift, bits, hist, total,
-                                   okey, opos, (uint8_t *)nullptr);
+        auto sort = [&](auto items) {
+            constexpr int J = decltype(items)::value;
+            for (uint32_t p = 0; p < passes; ++p, cur ^= 1) {
+                const uint32_t shift = p * bits;
+                uint2 *out = (uint2 *)(ws + w.place[cur ^ 1]);
+                const void *in = ws + w.place[cur];
+                auto pass = [&](auto hist_kernel, auto scatter_kernel, const void *src, unsigned extra, uint8_t *map) {
+                    hipLaunchKernelGGL(hist_kernel, dim3(tiles + extra), dim3(256), 0, s, src, t, n_rows, shift, bits, tiles, hist, ws + w.named);
+                    hipLaunchKernelGGL(rows_sort_scan_kernel, dim3(((1u << bits) + 63) / 64), dim3(1024), 0, s, hist, tiles, 1u << bits, total);
+                    hipLaunchKernelGGL(scatter_kernel, dim3(tiles), dim3(256), 0, s, src, t, n_rows, shift, bits, hist, total, out, map);
+                };
+                if (p == 0)
+                    with_id(id_bits, [&](auto zi) {
+                        using I = decltype(zi);
+                        pass(rows_sort_hist_kernel<J, true, I>, rows_sort_scatter_kernel<J, true, I>, d_ids, clear, named);
+                    });
+                else
+                    pass(rows_sort_hist_kernel<J, false, int32_t>, rows_sort_scatter_kernel<J, false, int32_t>, in, 0u, (uint8_t *)nullptr);
             }
-        }
+        };
+        if (w.tile == 1024) sort(std::integral_constant<int, 4>{});
+        else sort(std::integral_constant<int, 16>{});
     }
     // Columns per lane: 16 bytes of the gradients where addresses and dim allow, one element otherwise. Lanes per chunk:
     // the widest group that leaves few of its lanes without a column.
@@ -3473,8 +3501,7 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
     uint32_t lg = 6;
     while (lg > 3 && ((vpr + (1u << lg) - 1) >> lg << lg) > vpr + vpr / 8) --lg;
     GradArgs a;
-    a.key = (const uint32_t *)(ws + w.key[cur]);
-    a.pos = (const uint32_t *)(ws + w.pos[cur]);
+    a.place = (const uint2 *)(ws + w.place[cur]);
     a.t = t;
     a.chunks = w.chunks;
     a.R = w.R;
@@ -3497,7 +3524,12 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
             auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks + zero_blocks), dim3(256), 0, s, (const T *)d_grad_out, row_stride, a, (O *)d_grad); };
             if (vec) go(rows_grad_kernel<T, O, 16 / sizeof(T)>);
             else go(rows_grad_kernel<T, O, 1>);
-            if (a.chunks > 1) hipLaunchKernelGGL(rows_grad_join_kernel<O>, dim3(std::min<uint32_t>(a.chunks - 1, 1u << 16)), dim3(256), 0, s, a, (O *)d_grad);
+            if (a.chunks > 1) {
+                const bool four = dim % 4 == 0 && ((uintptr_t)d_grad & (4 * os - 1)) == 0;
+                const dim3 grid(std::min<uint32_t>((a.chunks + 7) / 8, 1u << 16), (dim + (four ? 255 : 63)) / (four ? 256 : 64));
+                if (four) hipLaunchKernelGGL((rows_grad_join_kernel<O, 4>), grid, dim3(256), 0, s, a, (O *)d_grad);
+                else hipLaunchKernelGGL((rows_grad_join_kernel<O, 1>), grid, dim3(256), 0, s, a, (O *)d_grad);
+            }
         });
     });
     HIP_TRY(hipGetLastError());

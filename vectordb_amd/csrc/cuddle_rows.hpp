@@ -75,24 +75,7 @@ __device__ __forceinline__ void load8(const T *row, uint32_t e0, uint32_t dim, f
     }
 }
 
-// Eight components to a row of outputs, those below `dim`.
-template <class T, bool VEC>
-__device__ __forceinline__ void store8(T *row, uint32_t e0, uint32_t dim, const float (&x)[8]) {
-    if (VEC && e0 + 8 <= dim) {
-        constexpr int N = 16 / sizeof(T);
-#pragma unroll
-        for (int p = 0; p < 8 / N; ++p) {
-            Pack<T, N> v;
-#pragma unroll
-            for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(x[p * N + i]);
-            *reinterpret_cast<Pack<T, N> *>(row + e0 + p * N) = v;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (e0 + i < dim) row[e0 + i] = from_f32<T>(x[i]);
-    }
-}
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------------------------
 // encoding
@@ -100,64 +83,79 @@ __device__ __forceinline__ void store8(T *row, uint32_t e0, uint32_t dim, const 
 // The code of x under scale s > 0 (inv = 1 / s, or 0 where that overflows): rint(x / s), exactly. s has 8 significant
 // bits and |n| <= 8, so n * s is exact; x - n * s is a multiple of the last place of x and no larger than x (or s),
 // so the fma returns it exactly and comparing it with s / 2 decides the rounding, whatever the estimate n was off by.
-__device__ __forceinline__ int32_t int4_code(float x, float s, float inv) {
+__device__ __forceinline__ float int4_code(float x, float s, float inv) {
     float n = rintf(inv != 0.f ? x * inv : x / s);
     n = fminf(fmaxf(n, -8.f), 8.f);
     const float r = __builtin_fmaf(-n, s, x), h = 0.5f * s;
     if (fabsf(r) > h || (fabsf(r) == h && ((int32_t)n & 1))) n += r > 0.f ? 1.f : -1.f;
-    return (int32_t)fminf(fmaxf(n, -7.f), 7.f);
+    return fminf(fmaxf(n, -7.f), 7.f);
 }
+constexpr float kInt4Magic = 12582912.f; // 1.5 * 2^23: x + this is rint(x) in the low bits of the sum
 
-// One block = one tile of 16 rows, 16 lanes per row; a lane has 8 consecutive components, the 16 lanes of a row two
-// units (128 components) per step. The group's largest magnitude is a reduction over G / 8 neighbouring lanes; the low
+// LPR lanes per row (16: one tile of 16 rows per block, 64: four rows); a lane has 8 consecutive components, so the lanes
+// of a row LPR / 8 units per step. The group's largest magnitude is a reduction over G / 8 neighbouring lanes; the low
 // and the high nibbles of a byte come from lanes 4 apart. Rows outside [first, first + count) are left alone.
 // sqnorm[r] = sum over groups of s^2 * sum c^2 in f64 (the integer sums are exact).
-// Bound by the read of the rows. grid = tiles touched (x stride), block 256.
-template <class T, bool VEC>
+// Bound by the read of the rows. grid = blocks of 256 / LPR rows (x stride), block 256.
+template <class T, bool VEC, int LPR>
 __global__ void __launch_bounds__(256)
 int4_encode_kernel(const T *x, uint64_t stride, uint64_t first, uint64_t count, uint32_t dim, uint32_t group, uint8_t *codes,
-                   uint16_t *scales, double *sqnorm, uint64_t tiles) {
-    const uint32_t units = int4_units(dim), gs = int4_gstride(dim, group), lane16 = threadIdx.x & 15, r = threadIdx.x >> 4;
-    const uint32_t jj = lane16 & 7;
-    for (uint64_t t = first / 16 + blockIdx.x; t < first / 16 + tiles; t += gridDim.x) {
-        const uint64_t row = t * 16 + r;
+                   uint16_t *scales, double *sqnorm, uint64_t blocks) {
+    constexpr uint32_t RPB = 256 / LPR, UPS = LPR / 8; // rows per block, units per step
+    const uint32_t units = int4_units(dim), gs = int4_gstride(dim, group), lr = threadIdx.x & (LPR - 1);
+    const uint32_t jj = lr & 7;
+    for (uint64_t bl = first / RPB + blockIdx.x; bl < first / RPB + blocks; bl += gridDim.x) {
+        const uint64_t row = bl * RPB + threadIdx.x / LPR, t = row >> 4;
+        const uint32_t r = (uint32_t)row & 15;
         const bool act = row >= first && row < first + count;
         const T *src = x + (act ? row - first : 0) * stride;
         double sq = 0.0;
-        for (uint32_t u0 = 0; u0 < units; u0 += 2) {
-            const uint32_t u = u0 + (lane16 >> 3), e0 = u * kInt4Unit + jj * 8;
+        float next[8]; // the next step's components are on their way while these are worked on
+        if (act) load8<T, VEC>(src, (lr >> 3) * kInt4Unit + jj * 8, dim, next);
+        for (uint32_t u0 = 0; u0 < units; u0 += UPS) {
+            const uint32_t u = u0 + (lr >> 3), e0 = u * kInt4Unit + jj * 8;
             float v[8];
-            if (act)
-                load8<T, VEC>(src, e0, dim, v);
-            else
-                for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            float a = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float m = fabsf(v[i]);
-                a = fmaxf(a, m <= 3.4028234663852886e38f ? m : __builtin_huge_valf()); // NaN counts as infinite
-            }
-            a = fmaxf(a, __shfl_xor(a, 1, 64));
-            a = fmaxf(a, __shfl_xor(a, 2, 64));
-            if (group >= 64) a = fmaxf(a, __shfl_xor(a, 4, 64));
-            if (group >= 128) a = fmaxf(a, __shfl_xor(a, 8, 64));
-            const bool bad = a > 3.4028234663852886e38f;
-            const uint16_t sb = bad ? (uint16_t)0x7FC0u : f32_to_bf16(a / 7.0f);
+            for (int i = 0; i < 8; ++i) v[i] = act ? next[i] : 0.f;
+            if (act && u0 + UPS < units) load8<T, VEC>(src, e0 + UPS * kInt4Unit, dim, next);
+            uint32_t ab = 0; // largest magnitude by its bits: infinities and NaN are above every number
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ab = max(ab, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+            ab = max(ab, (uint32_t)__shfl_xor((int)ab, 1, 64));
+            ab = max(ab, (uint32_t)__shfl_xor((int)ab, 2, 64));
+            if (group >= 64) ab = max(ab, (uint32_t)__shfl_xor((int)ab, 4, 64));
+            if (group >= 128) ab = max(ab, (uint32_t)__shfl_xor((int)ab, 8, 64));
+            const bool bad = ab >= 0x7F800000u;
+            const uint16_t sb = bad ? (uint16_t)0x7FC0u : f32_to_bf16(__uint_as_float(ab) / 7.0f);
             const float s = bf16_to_f32(sb);
+            // s of a normal size: |x| / s <= 7 (1 + 2^-8), so rint gives at most 7 and only remainders of half a step or
+            // more need the exact decision
             const float inv = s >= 1e-30f ? 1.0f / s : 0.f;
-            int32_t c[8], c2 = 0;
+            float mg[8], worst = 0.f, c2 = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                c[i] = (bad || s == 0.f) ? 0 : int4_code(v[i], s, inv);
-                c2 += c[i] * c[i];
+                mg[i] = __builtin_fmaf(v[i], inv, kInt4Magic);
+                const float n = mg[i] - kInt4Magic;
+                worst = fmaxf(worst, fabsf(__builtin_fmaf(-n, s, v[i])));
+                c2 = __builtin_fmaf(n, n, c2);
+            }
+            if (bad || inv == 0.f || worst >= 0.5f * s) {
+                c2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float n = (bad || s == 0.f) ? 0.f : int4_code(v[i], s, inv);
+                    mg[i] = n + kInt4Magic;
+                    c2 = __builtin_fmaf(n, n, c2);
+                }
             }
             sq = __builtin_fma((double)s * (double)s, (double)c2, sq);
-            uint32_t p0 = 0, p1 = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                p0 |= ((uint32_t)c[i] & 15u) << (8 * i);
-                p1 |= ((uint32_t)c[i + 4] & 15u) << (8 * i);
-            }
+            // the low nibbles of the sums are the codes: bytes 0 of four of them side by side
+            auto pack = [&](int i) {
+                const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(mg[i + 1]), __float_as_uint(mg[i]), 0x0C0C0400u);
+                const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(mg[i + 3]), __float_as_uint(mg[i + 2]), 0x04000C0Cu);
+                return (lo | hi) & 0x0F0F0F0Fu;
+            };
+            const uint32_t p0 = pack(0), p1 = pack(4);
             const uint32_t q0 = (uint32_t)__shfl_xor((int)p0, 4, 64), q1 = (uint32_t)__shfl_xor((int)p1, 4, 64);
             if (act && u < units) {
                 if (jj < 4)
@@ -167,13 +165,13 @@ int4_encode_kernel(const T *x, uint64_t stride, uint64_t first, uint64_t count, 
             }
         }
         // padding groups of the scales' row that no lane above stands for
-        if (act && lane16 < 8) {
-            const uint32_t g = (units * kInt4Unit + group - 1) / group + lane16;
+        if (act && lr < 8) {
+            const uint32_t g = (units * kInt4Unit + group - 1) / group + lr;
             if (g < gs) scales[row * gs + g] = 0;
         }
 #pragma unroll
-        for (int m = 1; m < 16; m <<= 1) sq += __shfl_xor(sq, m, 64);
-        if (act && lane16 == 0) sqnorm[row] = sq;
+        for (int m = 1; m < LPR; m <<= 1) sq += __shfl_xor(sq, m, 64);
+        if (act && lr == 0) sqnorm[row] = sq;
     }
 }
 
@@ -188,63 +186,94 @@ __device__ __forceinline__ uint64_t row_of_id(const I *ids, uint64_t t, uint64_t
     return i >= 0 && (uint64_t)i < n ? (uint64_t)i : kNoRow;
 }
 
-// out[t] = scale * table[ids[t]]; a block takes `rpb` outputs at a time and its threads the pieces of their rows, N
-// elements each. Bound by the writes (and the reads where the rows are not found in a cache).
+// out[t] = scale * table[ids[t]]. A thread has one piece of N elements (column blockIdx.y * w + ...) of every rpi-th of
+// the block's rpb outputs, four of them in flight: ids, then rows, then the stores. Bound by the writes (and by the reads
+// where the rows are not found in a cache).
 template <class T, class I, int N>
 __global__ void __launch_bounds__(256)
-rows_lookup_kernel(const T *table, uint64_t stride, uint64_t n, uint32_t dim, const I *ids, uint64_t n_ids, float scale, T *out, uint32_t rpb) {
-    const uint32_t ppr = (dim + N - 1) / N;
+rows_lookup_kernel(const T *table, uint64_t stride, uint64_t n, uint32_t dim, const I *ids, uint64_t n_ids, float scale, T *out, uint32_t w, uint32_t rpi,
+                   uint32_t rpb) {
+    const uint32_t rr = threadIdx.x / w, col = (blockIdx.y * w + threadIdx.x - rr * w) * N;
+    if (rr >= rpi || col >= dim) return;
+    constexpr int U = 4;
     for (uint64_t t0 = (uint64_t)blockIdx.x * rpb; t0 < n_ids; t0 += (uint64_t)gridDim.x * rpb) {
-        const uint32_t items = (uint32_t)min((uint64_t)rpb, n_ids - t0) * ppr;
-        for (uint32_t it = threadIdx.x; it < items; it += 256) {
-            const uint32_t rr = it / ppr, p = it - rr * ppr;
-            const uint64_t t = t0 + rr, row = row_of_id(ids, t, n);
-            Pack<T, N> v;
-            if (row != kNoRow) {
-                v = *reinterpret_cast<const Pack<T, N> *>(table + row * stride + (uint64_t)p * N);
+        const uint64_t te = min(t0 + rpb, n_ids);
+        for (uint64_t t1 = t0 + rr; t1 < te; t1 += U * rpi) {
+            uint64_t row[U];
+            Pack<T, N> v[U];
 #pragma unroll
-                for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(to_f32(v.v[i]) * scale);
-            } else {
+            for (int u = 0; u < U; ++u) row[u] = t1 + u * rpi < te ? row_of_id(ids, t1 + u * rpi, n) : kNoRow;
 #pragma unroll
-                for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(0.f);
+            for (int u = 0; u < U; ++u) {
+                if (row[u] != kNoRow)
+                    v[u] = *reinterpret_cast<const Pack<T, N> *>(table + row[u] * stride + col);
+                else
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[u].v[i] = from_f32<T>(0.f);
             }
-            *reinterpret_cast<Pack<T, N> *>(out + t * dim + (uint64_t)p * N) = v;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (t1 + u * rpi >= te) continue;
+                if (row[u] != kNoRow)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[u].v[i] = from_f32<T>(to_f32(v[u].v[i]) * scale);
+                *reinterpret_cast<Pack<T, N> *>(out + (t1 + u * rpi) * dim + col) = v[u];
+            }
         }
     }
 }
 
-// The same from 4-bit rows: a piece is 8 components, one nibble of each of 8 bytes (lanes 4 apart share the bytes).
-// s * c has 12 significant bits, so only the product with `scale` and the rounding to the output's type round.
-// ids == nullptr: rows 0 .. n_ids - 1 in order.
-template <class T, class I, bool VEC>
+// The same from 4-bit rows: a piece is what 16 bytes of output hold, one nibble of each of N bytes (threads 32 components
+// apart share the bytes). s * c has 12 significant bits, so only the product with `scale` and the rounding to the output's
+// type round. ids == nullptr: rows 0 .. n_ids - 1 in order, one at a time (U = 1), written without a claim to a cache.
+template <class T, class I, bool VEC, int U>
 __global__ void __launch_bounds__(256)
 int4_lookup_kernel(const uint8_t *codes, const uint16_t *scales, uint64_t n, uint32_t dim, uint32_t group, const I *ids, uint64_t n_ids, float scale,
-                   T *out, uint32_t rpb) {
-    const uint32_t units = int4_units(dim), gs = int4_gstride(dim, group), ppr = (dim + 7) / 8;
+                   T *out, uint32_t w, uint32_t rpi, uint32_t rpb) {
+    constexpr int N = 16 / sizeof(T), W = N / 4; // components, words of codes
+    const uint32_t units = int4_units(dim), gs = int4_gstride(dim, group), rr = threadIdx.x / w, e0 = (blockIdx.y * w + threadIdx.x - rr * w) * N;
+    if (rr >= rpi || e0 >= dim) return;
+    const uint32_t e6 = e0 & 63, code_at = (e0 >> 6) * kInt4UnitBytes + (e6 & 31), g = e0 / group, up = e6 < 32 ? 4 : 0;
     for (uint64_t t0 = (uint64_t)blockIdx.x * rpb; t0 < n_ids; t0 += (uint64_t)gridDim.x * rpb) {
-        const uint32_t items = (uint32_t)min((uint64_t)rpb, n_ids - t0) * ppr;
-        for (uint32_t it = threadIdx.x; it < items; it += 256) {
-            const uint32_t rr = it / ppr, p = it - rr * ppr;
-            const uint64_t t = t0 + rr, row = ids ? row_of_id(ids, t, n) : t;
-            float x[8];
-            if (row != kNoRow) {
-                const uint32_t u = p >> 3, jj = p & 7;
-                uint2 w = *reinterpret_cast<const uint2 *>(codes + ((row >> 4) * units + u) * kInt4UnitBytes + (uint32_t)(row & 15) * 32 + (jj & 3) * 8);
-                if (jj < 4) {
-                    w.x <<= 4;
-                    w.y <<= 4;
-                }
-                const float s = bf16_to_f32(scales[row * gs + p * 8 / group]);
+        const uint64_t te = min(t0 + rpb, n_ids);
+        for (uint64_t t1 = t0 + rr; t1 < te; t1 += U * rpi) {
+            uint64_t row[U];
+            Pack<uint32_t, W> c[U];
+            uint16_t sb[U];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = s * (float)((int32_t)(w.x << (24 - 8 * i)) >> 28) * scale;
-                    x[i + 4] = s * (float)((int32_t)(w.y << (24 - 8 * i)) >> 28) * scale;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = 0.f;
+            for (int u = 0; u < U; ++u) {
+                const uint64_t t = t1 + u * rpi;
+                row[u] = t >= te ? kNoRow : ids ? row_of_id(ids, t, n) : t;
             }
-            store8<T, VEC>(out + t * dim, p * 8, dim, x);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) c[u].v[i] = 0;
+                sb[u] = 0;
+                if (row[u] != kNoRow) {
+                    c[u] = *reinterpret_cast<const Pack<uint32_t, W> *>(codes + (row[u] >> 4) * units * kInt4UnitBytes + (uint32_t)(row[u] & 15) * 32 + code_at);
+                    sb[u] = scales[row[u] * gs + g];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (t1 + u * rpi >= te) continue;
+                const float s = bf16_to_f32(sb[u]);
+                Pack<T, N> o;
+#pragma unroll
+                for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(s * (float)((int32_t)((c[u].v[i / 4] << up) << (24 - 8 * (i & 3))) >> 28) * scale);
+                T *dst = out + (t1 + u * rpi) * dim + e0;
+                if (VEC && U == 1) {
+                    u32x4_t b;
+                    __builtin_memcpy(&b, &o, 16);
+                    __builtin_nontemporal_store(b, reinterpret_cast<u32x4_t *>(dst));
+                } else if (VEC)
+                    *reinterpret_cast<Pack<T, N> *>(dst) = o;
+                else
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (e0 + i < dim) dst[i] = o.v[i];
+            }
         }
     }
 }
@@ -309,10 +338,17 @@ int4_query_kernel(const T *queries, uint32_t nq, uint32_t dim, uint32_t units, u
     }
 }
 
+// 1 / sqrt(z) in f64: the hardware's estimate, refined twice (each step squares its error and trebles a half of it).
+__device__ __forceinline__ double inv_sqrt(double z) {
+    double y = __builtin_amdgcn_rsq(z);
+    y = __builtin_fma(y * 0.5, __builtin_fma(-z * y, y, 1.0), y);
+    return __builtin_fma(y * 0.5, __builtin_fma(-z * y, y, 1.0), y);
+}
+
 // distance from the product p = scale * sum: l2 |x|^2 + |q|^2 - 2p, cosine 1 - p / (|x||q|), dot -p; in f64, rounded once.
 __device__ __forceinline__ float int4_finish(uint32_t metric, double sum, double scale, double xsq, double qsq) {
     if (metric == kMetricDot) return (float)(-scale * sum);
-    if (metric == kMetricCosine) return (float)(1.0 - scale * sum / (sqrt(xsq) * sqrt(qsq)));
+    if (metric == kMetricCosine) return (float)__builtin_fma(-scale * sum, inv_sqrt(xsq * qsq), 1.0); // the squares of f32 norms multiply within f64's range
     const float d = (float)__builtin_fma(-2.0 * scale, sum, xsq + qsq);
     return d < 0.f ? 0.f : d; // the three terms of a row next to the query round apart
 }
@@ -439,7 +475,7 @@ __device__ __forceinline__ Int4Test int4_test(uint32_t metric, uint32_t tau, con
 __device__ __forceinline__ float int4_test_row(uint32_t metric, double xsq) {
     if (metric == kMetricDot) return 0.f;
     if (!(xsq < 1e30 && xsq > 1e-30)) return __builtin_nanf("");
-    return metric == kMetricCosine ? (float)(1.0 / sqrt(xsq)) : (float)(xsq * (1.0 - 1.0 / (1 << 19)));
+    return metric == kMetricCosine ? (float)inv_sqrt(xsq) : (float)(xsq * (1.0 - 1.0 / (1 << 19)));
 }
 template <uint32_t METRIC>
 __device__ __forceinline__ bool int4_beyond(double hi, float lo, const Int4Test &q, float row) {
@@ -940,7 +976,7 @@ __device__ __forceinline__ uint32_t wave_rank(uint32_t d, bool in, uint32_t bits
 constexpr uint32_t kSortSmall = 3840; // what 64 KB of LDS hold beside the counters
 template <class I>
 __global__ void __launch_bounds__(1024)
-rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passes, uint32_t *okey, uint32_t *opos, void *zero, uint64_t zero_bytes) {
+rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passes, uint2 *out, void *zero, uint64_t zero_bytes) {
     if (blockIdx.x) {
         zero_share(zero, zero_bytes, blockIdx.x - 1, gridDim.x - 1);
         return;
@@ -991,18 +1027,17 @@ rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passe
         }
         __syncthreads();
     }
-    for (uint32_t i = tid; i < t; i += 1024) {
-        okey[i] = key[cur][i];
-        opos[i] = pos[cur][i];
-    }
+    for (uint32_t i = tid; i < t; i += 1024) out[i] = make_uint2(key[cur][i], pos[cur][i]);
 }
 
-// More places: per pass (up to 10 bits) a histogram per tile of 4096 places, the histograms' prefix sums, the scatter.
+// More places: per pass (up to 10 bits) a histogram per tile of J * 256 places, the histograms' prefix sums, the scatter.
+// J = 4 up to a million places (the tiles' waves rank their places one 64 after the other: 64K places 15 us with J = 16,
+// 6 us with 4), 16 beyond (the histograms grow with the tiles).
 // The first pass reads the ids themselves. The first histogram launch also clears the map of rows that ids name
 // (one byte each), the first scatter fills it in; the gradient kernel zeroes the rows it does not hold.
-constexpr uint32_t kSortTile = 4096, kSortMaxBits = 10;
+constexpr uint32_t kSortMaxBits = 10;
 
-template <bool FIRST, class I>
+template <int J, bool FIRST, class I>
 __global__ void __launch_bounds__(256)
 rows_sort_hist_kernel(const void *src, uint32_t t, uint64_t n_rows, uint32_t shift, uint32_t bits, uint32_t tiles, uint32_t *hist, uint8_t *named) {
     if (blockIdx.x >= tiles) {
@@ -1013,12 +1048,12 @@ rows_sort_hist_kernel(const void *src, uint32_t t, uint64_t n_rows, uint32_t shi
     const uint32_t bins = 1u << bits;
     for (uint32_t i = threadIdx.x; i < bins; i += 256) h[i] = 0;
     __syncthreads();
-    const uint32_t b = blockIdx.x * kSortTile;
+    const uint32_t b = blockIdx.x * (J * 256);
 #pragma unroll
-    for (uint32_t j = 0; j < kSortTile / 256; ++j) {
+    for (uint32_t j = 0; j < J; ++j) {
         const uint32_t i = b + j * 256 + threadIdx.x;
         if (i < t) {
-            const uint32_t k = FIRST ? grad_key(static_cast<const I *>(src), i, n_rows) : static_cast<const uint32_t *>(src)[i];
+            const uint32_t k = FIRST ? grad_key(static_cast<const I *>(src), i, n_rows) : static_cast<const uint2 *>(src)[i].x;
             atomicAdd(&h[(k >> shift) & (bins - 1)], 1u);
         }
     }
@@ -1035,6 +1070,7 @@ rows_sort_scan_kernel(uint32_t *hist, uint32_t tiles, uint32_t bins, uint32_t *t
     const uint32_t per = (tiles + 15) / 16, b = min(w * per, tiles), e = min(b + per, tiles);
     uint32_t sum = 0;
     if (d < bins)
+#pragma unroll 8
         for (uint32_t i = b; i < e; ++i) sum += hist[(uint64_t)i * bins + d];
     part[w][lane] = sum;
     __syncthreads();
@@ -1042,17 +1078,23 @@ rows_sort_scan_kernel(uint32_t *hist, uint32_t tiles, uint32_t bins, uint32_t *t
     for (uint32_t v = 0; v < w; ++v) run += part[v][lane];
     if (d >= bins) return;
     if (w == 15) total[d] = run + sum;
-    for (uint32_t i = b; i < e; ++i) {
-        const uint32_t v = hist[(uint64_t)i * bins + d];
-        hist[(uint64_t)i * bins + d] = run;
-        run += v;
+    for (uint32_t i0 = b; i0 < e; i0 += 8) { // eight reads in flight
+        uint32_t v[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) v[j] = i0 + j < e ? hist[(uint64_t)(i0 + j) * bins + d] : 0u;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+            if (i0 + j < e) {
+                hist[(uint64_t)(i0 + j) * bins + d] = run;
+                run += v[j];
+            }
     }
 }
 
-template <bool FIRST, class I>
+template <int J, bool FIRST, class I>
 __global__ void __launch_bounds__(256)
-rows_sort_scatter_kernel(const void *src, const uint32_t *pos, uint32_t t, uint64_t n_rows, uint32_t shift, uint32_t bits, const uint32_t *hist,
-                         const uint32_t *total, uint32_t *okey, uint32_t *opos, uint8_t *named) {
+rows_sort_scatter_kernel(const void *src, uint32_t t, uint64_t n_rows, uint32_t shift, uint32_t bits, const uint32_t *hist,
+                         const uint32_t *total, uint2 *out, uint8_t *named) {
     __shared__ uint32_t off[4][1u << kSortMaxBits];
     __shared__ uint32_t tot[(1u << kSortMaxBits) + 1];
     const uint32_t tid = threadIdx.x, w = tid >> 6, lane = tid & 63, bins = 1u << bits;
@@ -1061,14 +1103,21 @@ rows_sort_scatter_kernel(const void *src, const uint32_t *pos, uint32_t t, uint6
         tot[i] = total[i];
     }
     __syncthreads();
-    const uint32_t b = blockIdx.x * kSortTile + w * (kSortTile / 4);
-    uint32_t k[kSortTile / 256], ps[kSortTile / 256];
+    const uint32_t b = blockIdx.x * (J * 256) + w * (J * 64);
+    uint32_t k[J], ps[J];
 #pragma unroll
-    for (uint32_t j = 0; j < kSortTile / 256; ++j) {
+    for (uint32_t j = 0; j < J; ++j) {
         const uint32_t i = b + j * 64 + lane;
         const bool in = i < t;
-        k[j] = in ? (FIRST ? grad_key(static_cast<const I *>(src), i, n_rows) : static_cast<const uint32_t *>(src)[i]) : 0u;
-        ps[j] = in ? (FIRST ? i : pos[i]) : 0u;
+        k[j] = ps[j] = 0u;
+        if (in && FIRST) {
+            k[j] = grad_key(static_cast<const I *>(src), i, n_rows);
+            ps[j] = i;
+        } else if (in) {
+            const uint2 e = static_cast<const uint2 *>(src)[i];
+            k[j] = e.x;
+            ps[j] = e.y;
+        }
         if (in) atomicAdd(&off[w][(k[j] >> shift) & (bins - 1)], 1u);
         if (FIRST && named && in && k[j] < n_rows) named[k[j]] = 1;
     }
@@ -1085,13 +1134,10 @@ rows_sort_scatter_kernel(const void *src, const uint32_t *pos, uint32_t t, uint6
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t j = 0; j < kSortTile / 256; ++j) {
+    for (uint32_t j = 0; j < J; ++j) {
         const bool in = b + j * 64 + lane < t;
         const uint32_t at = wave_rank((k[j] >> shift) & (bins - 1), in, bits, off[w]);
-        if (in) {
-            okey[at] = k[j];
-            opos[at] = ps[j];
-        }
+        if (in) out[at] = make_uint2(k[j], ps[j]);
     }
 }
 
@@ -1116,7 +1162,7 @@ __device__ __forceinline__ void grad_store(O *o, const float (&sum)[V], float sc
 // Blocks from `blocks` on zero the rows that no id names. Bound by the read of the gradients, a row at a time, and the
 // write of the table's gradient.
 struct GradArgs {
-    const uint32_t *key, *pos;
+    const uint2 *place; // (row, position in the list of ids), sorted
     uint32_t t, chunks, R, lg, cbs, blocks; // cbs: column blocks of L * V
     uint64_t n_rows;
     uint32_t dim;
@@ -1153,8 +1199,8 @@ rows_grad_kernel(const T *g, uint64_t stride, GradArgs a, O *grad) {
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
-    uint32_t cur = a.key[begin];
-    bool cont = begin > 0 && a.key[begin - 1] == cur;
+    uint32_t cur = a.place[begin].x;
+    bool cont = begin > 0 && a.place[begin - 1].x == cur;
     auto flush = [&](bool open) {
         if (cur >= a.n_rows) return;
         if (!cont && !open) {
@@ -1173,8 +1219,9 @@ rows_grad_kernel(const T *g, uint64_t stride, GradArgs a, O *grad) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t j = min(j0 + u, end - 1);
-            k[u] = a.key[j];
-            v[u] = *reinterpret_cast<const Pack<T, V> *>(g + (uint64_t)a.pos[j] * stride + col);
+            const uint2 e = a.place[j];
+            k[u] = e.x;
+            v[u] = *reinterpret_cast<const Pack<T, V> *>(g + (uint64_t)e.y * stride + col);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -1190,43 +1237,76 @@ rows_grad_kernel(const T *g, uint64_t stride, GradArgs a, O *grad) {
             for (int i = 0; i < V; ++i) sum[i] += to_f32(v[u].v[i]);
         }
     }
-    flush(end < a.t && a.key[end] == cur);
+    flush(end < a.t && a.place[end].x == cur);
 }
 
-// One block per chunk; it works where a run opens in the chunk and goes on beyond it: the parts of the run, in order, a
-// quarter of them per wave, 64 columns at a time. The last chunk of the run is found by bisection (keys are sorted).
-template <class O>
+// The cut runs. A block looks at 8 chunks; where a run opens in one and goes on beyond it, its four waves add the run's
+// parts up, a quarter of them each in order, 64 * V columns at a time (grid.y), and the quarters in order. The last chunk
+// of the run is found by bisection (keys are sorted).
+template <class O, int V>
 __global__ void __launch_bounds__(256)
 rows_grad_join_kernel(GradArgs a, O *grad) {
-    __shared__ float s_part[4][64];
-    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (uint32_t c = blockIdx.x; c + 1 < a.chunks; c += gridDim.x) {
-        const uint32_t begin = c * a.R, end = begin + a.R; // not the last chunk: it is full
-        const uint32_t row = a.key[end - 1];
-        if (row >= a.n_rows || a.key[end] != row) continue;
-        if (a.key[begin] == row && begin > 0 && a.key[begin - 1] == row) continue; // opened earlier
-        uint32_t lo = c + 1, hi = a.chunks - 1; // the last chunk whose first key is the row
-        while (lo < hi) {
-            const uint32_t m = (lo + hi + 1) / 2;
-            if (a.key[m * a.R] == row) lo = m;
-            else hi = m - 1;
+    __shared__ float s_part[4][64 * V];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = (blockIdx.y * 64 + lane) * V;
+    const bool have = col < a.dim; // V divides dim
+    for (uint32_t c0 = blockIdx.x * 8; c0 + 1 < a.chunks; c0 += gridDim.x * 8) {
+        // lane j: the run that opens in chunk c0 + j and goes on, its row and last chunk
+        uint32_t row = 0xFFFFFFFFu, last = 0;
+        const uint32_t c = c0 + (lane & 7);
+        if (c + 1 < a.chunks) {
+            const uint32_t begin = c * a.R, end = begin + a.R; // not the last chunk: it is full
+            row = a.place[end - 1].x;
+            const bool opens = !(a.place[begin].x == row && begin > 0 && a.place[begin - 1].x == row);
+            if (row >= a.n_rows || a.place[end].x != row || !opens) row = 0xFFFFFFFFu;
+            if (row != 0xFFFFFFFFu) {
+                uint32_t lo = c + 1, hi = a.chunks - 1; // the last chunk whose first key is the row
+                for (uint32_t step = 1; lo + step <= hi; step *= 2) { // most runs end in the next chunk
+                    if (a.place[(lo + step) * a.R].x != row) {
+                        hi = lo + step - 1;
+                        break;
+                    }
+                    lo += step;
+                }
+                while (lo < hi) {
+                    const uint32_t m = (lo + hi + 1) / 2;
+                    if (a.place[m * a.R].x == row) lo = m;
+                    else hi = m - 1;
+                }
+                last = lo;
+            }
         }
-        const uint32_t parts = lo - c, per = (parts + 3) / 4, p0 = min(w * per, parts), p1 = min(p0 + per, parts);
-        for (uint32_t col0 = 0; col0 < a.dim; col0 += 64) {
-            const uint32_t col = col0 + lane;
-            float sum = 0.f;
-            if (col < a.dim) {
-                if (w == 0) sum = a.part[((uint64_t)c * 2 + 1) * a.dim + col];
+        uint64_t todo = __ballot(row != 0xFFFFFFFFu && lane < 8); // the same in every wave
+        while (todo) {
+            const uint32_t j = (uint32_t)__ffsll((unsigned long long)todo) - 1;
+            todo &= todo - 1;
+            const uint32_t rr = (uint32_t)__builtin_amdgcn_readlane((int)row, (int)j), cl = (uint32_t)__builtin_amdgcn_readlane((int)last, (int)j);
+            const uint32_t cc = c0 + j, parts = cl - cc, per = (parts + 3) / 4, p0 = min(w * per, parts), p1 = min(p0 + per, parts);
+            float sum[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] = 0.f;
+            if (have) {
+                if (w == 0) {
+                    const Pack<float, V> v = *reinterpret_cast<const Pack<float, V> *>(a.part + ((uint64_t)cc * 2 + 1) * a.dim + col);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum[i] = v.v[i];
+                }
 #pragma unroll 8
-                for (uint32_t p = p0; p < p1; ++p) sum += a.part[(uint64_t)(c + 1 + p) * 2 * a.dim + col];
+                for (uint32_t p = p0; p < p1; ++p) {
+                    const Pack<float, V> v = *reinterpret_cast<const Pack<float, V> *>(a.part + (uint64_t)(cc + 1 + p) * 2 * a.dim + col);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum[i] += v.v[i];
+                }
             }
-            __syncthreads(); // the sums of the columns before have been read
-            s_part[w][lane] = sum;
-            __syncthreads();
-            if (w == 0 && col < a.dim) {
-                const float one[1] = {((s_part[0][lane] + s_part[1][lane]) + s_part[2][lane]) + s_part[3][lane]};
-                grad_store<O, 1>(grad + (uint64_t)row * a.dim + col, one, a.scale, a.accumulate);
+            if (parts > 1) { // not the first wave's work alone
+                __syncthreads(); // the sums before have been read
+#pragma unroll
+                for (int i = 0; i < V; ++i) s_part[w][lane * V + i] = sum[i];
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    sum[i] = ((s_part[0][lane * V + i] + s_part[1][lane * V + i]) + s_part[2][lane * V + i]) + s_part[3][lane * V + i];
             }
+            if (w == 0 && have) grad_store<O, V>(grad + (uint64_t)rr * a.dim + col, sum, a.scale, a.accumulate);
         }
     }
 }

@@ -2913,6 +2913,10 @@ struct DeviceGuard { // the calls below leave the caller's current device as it 
             (void)hipGetLastError();
             prev = -1;
         }
+        if (prev >= 0 && prev == device_id) {
+            prev = -1; // nothing to put back
+            return CUDDLE_OK;
+        }
         return use_device(device_id);
     }
     ~DeviceGuard() {
@@ -2980,6 +2984,11 @@ template <class F> void with_id(uint32_t bits, F f) {
 constexpr size_t kAlign = 256;
 size_t round_ws(size_t b) { return (b + kAlign - 1) & ~(kAlign - 1); }
 
+constexpr uint32_t int4_lds_kb(int qt) { return qt >= 3 ? 144u : 64u; } // digits per block: one block of 8 waves per CU, or two of 4 and more
+// Up to four queries whose digits fit a block's LDS: the distance kernel makes them itself. A round of a call is fused if
+// its queries are this few, so a call of more queries lays out room for digits also for a last, smaller round.
+bool int4_fused(uint64_t nq, uint32_t dim) { return nq <= 4 && (int4_units(dim) + 7) / 8 * 8 <= int4_lds_kb(1); }
+
 // Work space of the distance and search calls: the queries' digits, and for a search the distances of `qc` queries and
 // two selection buffers.
 struct Int4Ws {
@@ -2994,6 +3003,17 @@ constexpr uint64_t kInt4MaxRound = 32768;          // queries per round (the lau
 // launches cost about 30 us).
 constexpr uint64_t kInt4SampleFrom = 32ull << 20;
 
+// Items per block of a selection level: fewer where that fills the chip sooner (50 000 items, one query, k = 100: 16 us in 7
+// blocks, 6 in 25), as long as one more level answers and a chunk is several times what it keeps.
+uint32_t top_chunk(uint64_t items, uint32_t nq, uint32_t k) {
+    const uint64_t fits = 3072 / k; // parts that the last level takes without becoming the longer one
+    for (uint32_t chunk : {1024u, 2048u, 4096u}) {
+        const uint64_t parts = (items + chunk - 1) / chunk;
+        if (chunk >= 8 * k && parts <= fits && parts * nq <= 1024) return chunk;
+    }
+    return kTopChunk;
+}
+
 Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
     Int4Ws w;
     uint64_t qc = std::min<uint64_t>(nq, kInt4MaxRound);
@@ -3006,12 +3026,15 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
         at += round_ws(b);
         return p;
     };
-    w.dig = take(quartets * int4_units(dim) * 1024);
-    w.info = take(quartets * 4 * sizeof(Int4Query));
+    if (!int4_fused(nq, dim)) {
+        w.dig = take(quartets * int4_units(dim) * 1024);
+        w.info = take(quartets * 4 * sizeof(Int4Query));
+    }
     if (k) {
         w.dist = take((size_t)qc * n * 4);
         if (parts > 1) {
-            w.sel[0] = take((size_t)qc * parts * k * 8);
+            const uint64_t first = std::max<uint64_t>(parts * k, std::min<uint64_t>(kTopChunk, (n + 1023) / 1024 * k)); // smaller chunks: at most kTopChunk items
+            w.sel[0] = take((size_t)qc * first * 8);
             w.sel[1] = take((size_t)qc * ((parts * k + kTopChunk - 1) / kTopChunk) * k * 8);
         }
         // k of a sample of S rows bound k n / S of all: enough to expect 512 candidates, at most a sixteenth of the
@@ -3033,8 +3056,6 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
 // Launch shapes of the distance kernel. One quartet of queries: codes are the bound, so many of them are requested at a
 // time (16 pieces of 512 bytes per wave). More: QT quartets per wave, the count among those built that costs least,
 // pairs of (row, query) at about 27 cycles and the unpacking of the codes, once per QT, at about as much.
-constexpr uint32_t int4_lds_kb(int qt) { return qt >= 3 ? 144u : 64u; } // digits per block: one block of 8 waves per CU, or two of 4 and more
-
 template <int G, int QT, int T, int P, bool FUSED, bool NT, class TQ>
 void int4_launch(Int4DistArgs a, hipStream_t s) {
     constexpr uint32_t NW = int4_block(QT) / 64;
@@ -3135,7 +3156,7 @@ Int4DistArgs int4_prepare(const cuddle_int4_rows *r, const void *queries, uint32
     a.nq = nq;
     a.metric = metric;
     a.stiles = (r->n + 15) / 16;
-    fused = nq <= 4 && (a.units + 7) / 8 * 8 <= int4_lds_kb(1);
+    fused = int4_fused(nq, r->dim);
     if (!fused)
         with_type(type, [&](auto z) {
             using T = decltype(z);
@@ -3330,10 +3351,11 @@ extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows,
         uint64_t stride = rows->n, items = rows->n;
         int level = 0;
         for (; items > kTopChunk; ++level) {
-            const uint64_t parts = (items + kTopChunk - 1) / kTopChunk;
+            const uint32_t chunk = top_chunk(items, nq, k);
+            const uint64_t parts = (items + chunk - 1) / chunk;
             uint64_t *out = (uint64_t *)(ws + w.sel[level & 1]);
             auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)parts, nq), dim3(kTopThreads), 0, s, in, stride, items, k, out, (const uint32_t *)cnt, kTopChunk);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)parts, nq), dim3(kTopThreads), 0, s, in, stride, items, k, chunk, out, (const uint32_t *)cnt, kTopChunk);
             };
             if (level == 0) go(int4_topk_level_kernel<true>);
             else go(int4_topk_level_kernel<false>);

@@ -738,12 +738,12 @@ constexpr uint32_t kTopThreads = 512;
 struct TopkLds {
     uint32_t hist[256];
     uint32_t lo[kTopThreads / 64], hi[kTopThreads / 64];
-    uint32_t bin, rest;
+    uint32_t bin, rest, full;
     uint32_t wtmp[2 * kTopThreads / 64];
 };
 
-// The k-th smallest (1 <= k <= C) of the keys key(0) .. key(C - 1), and how many of those equal to it belong to the k
-// smallest. 8 bits at a time from the highest bit in which the keys differ: distances share their leading bits, and a
+// T and budget such that the k smallest (1 <= k <= C) of the keys key(0) .. key(C - 1) are those below T and `budget` of
+// those equal to T: T is the k-th smallest or, where nothing lies between, larger. 8 bits at a time from the highest bit in which the keys differ: distances share their leading bits, and a
 // histogram of those would be one counter that every thread adds to. All threads of a block of kTopThreads.
 template <class KeyFn>
 __device__ __forceinline__ void block_kth_key(uint32_t C, uint32_t k, KeyFn key, TopkLds &s, uint32_t &T, uint32_t &budget) {
@@ -786,33 +786,41 @@ __device__ __forceinline__ void block_kth_key(uint32_t C, uint32_t k, KeyFn key,
             const uint32_t incl = wave_inclusive_sum(c0 + c1 + c2 + c3);
             uint32_t run = incl - (c0 + c1 + c2 + c3);
             if (run < budget && budget <= incl) {
-                uint32_t bin = b;
-                if (run + c0 < budget) { run += c0; ++bin;
-                    if (run + c1 < budget) { run += c1; ++bin;
-                        if (run + c2 < budget) { run += c2; ++bin; } } }
+                uint32_t bin = b, c = c0;
+                if (run + c0 < budget) { run += c0; ++bin; c = c1;
+                    if (run + c1 < budget) { run += c1; ++bin; c = c2;
+                        if (run + c2 < budget) { run += c2; ++bin; c = c3; } } }
                 s.bin = bin;
                 s.rest = budget - run;
+                s.full = c == budget - run ? 1u : 0u;
             }
         }
         __syncthreads();
         prefix |= s.bin << shift;
         mask |= (bins - 1) << shift;
         budget = s.rest;
+        const bool full = s.full != 0;
         __syncthreads();
+        if (full) { // everything that starts with these digits is wanted: no need to know how it goes on
+            prefix |= ~mask;
+            budget = C;
+            break;
+        }
     }
     T = prefix;
 }
 
 // Level: from f32 distances (FIRST) or from the previous level's lists. in: [nq][in_stride]; out: [nq][parts][k].
-// redo: nullptr, or only queries that count more than `cap`. grid (parts, nq), block kTopThreads.
+// chunk <= kTopChunk items per block. redo: nullptr, or only queries that count more than `cap`. grid (parts, nq), block
+// kTopThreads.
 template <bool FIRST>
 __global__ void __launch_bounds__(kTopThreads)
-int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint32_t k, uint64_t *out, const uint32_t *redo, uint32_t cap) {
+int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint32_t k, uint32_t chunk, uint64_t *out, const uint32_t *redo, uint32_t cap) {
     __shared__ uint32_t keys[kTopChunk];
     __shared__ TopkLds s;
     if (redo && redo[blockIdx.y] <= cap) return;
-    const uint64_t base = (uint64_t)blockIdx.x * kTopChunk;
-    const uint32_t C = (uint32_t)min((uint64_t)kTopChunk, items - base), tid = threadIdx.x;
+    const uint64_t base = (uint64_t)blockIdx.x * chunk;
+    const uint32_t C = (uint32_t)min((uint64_t)chunk, items - base), tid = threadIdx.x;
     const float *df = static_cast<const float *>(in) + (uint64_t)blockIdx.y * in_stride + base;
     const uint64_t *dl = static_cast<const uint64_t *>(in) + (uint64_t)blockIdx.y * in_stride + base;
 #pragma unroll 8

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 from typing import List, Optional, Tuple
 
 import numpy as np
@@ -66,8 +67,8 @@ def _enter(dev: torch.device, stream, *inputs: torch.Tensor):
     return torch.cuda.stream(stream), index, C.c_void_p(stream.cuda_stream)
 
 
-def _workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
-    return torch.empty((max(int(nbytes), 1),), dtype=torch.uint8, device=dev)
+def _workspace(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
 
 
 class Int4Rows:
@@ -88,6 +89,7 @@ class Int4Rows:
         self._desc = _ffi.Int4RowsDesc(codes.data_ptr(), scales.data_ptr(), sqnorm.data_ptr(), n, dim, group)
 
     @staticmethod
+    @functools.lru_cache(maxsize=256)
     def _sizes(n: int, dim: int, group: int) -> Tuple[int, int]:
         nbytes, stride = C.c_uint64(0), C.c_uint32(0)
         _ffi.check(_ffi.lib().cuddle_int4_sizes(n, dim, group, C.byref(nbytes), C.byref(stride)))
@@ -155,10 +157,12 @@ class Int4Rows:
             raise ValueError("Query dimension mismatch")
         return _cuda(self.codes, q), _type_id(q.dtype)
 
-    def _ws(self, nq: int, k: int, dev: torch.device) -> Tuple[torch.Tensor, int]:
+    def _ws(self, nq: int, k: int, dev: torch.device):
+        """(tensor that keeps the work space, its address or None, bytes)"""
         need = C.c_uint64(0)
         _ffi.check(_ffi.lib().cuddle_int4_workspace(self.n, self.dim, nq, k, C.byref(need)))
-        return _workspace(need.value, dev), int(need.value)
+        ws = _workspace(need.value, dev)
+        return ws, None if ws is None else ws.data_ptr(), need.value
 
     def distances_device(self, queries: torch.Tensor, metric="l2", stream=None) -> torch.Tensor:
         """distance(query, row) of queries [nq, dim] (float32, float16, bfloat16) to every row: float32 [nq, n]."""
@@ -167,8 +171,8 @@ class Int4Rows:
         with ctx:
             q = queries.contiguous()
             out = torch.empty((q.shape[0], self.n), dtype=torch.float32, device=dev)
-            ws, need = self._ws(q.shape[0], 0, dev)
-            _ffi.check(_ffi.lib().cuddle_int4_distances_device(C.byref(self._desc), q.data_ptr(), kind, q.shape[0], m, out.data_ptr(), ws.data_ptr(), need,
+            ws, at, need = self._ws(q.shape[0], 0, dev)
+            _ffi.check(_ffi.lib().cuddle_int4_distances_device(C.byref(self._desc), q.data_ptr(), kind, q.shape[0], m, out.data_ptr(), at, need,
                                                                index, st))
         return out
 
@@ -181,12 +185,12 @@ class Int4Rows:
         with ctx:
             q = queries.contiguous()
             k = min(max(int(k), 0), 0xFFFFFFFF)  # refused by the library
-            ws, need = self._ws(nq, k, dev)
+            ws, at, need = self._ws(nq, k, dev)
             ids = torch.empty((nq, k), dtype=torch.int64, device=dev)
             dist = torch.empty((nq, k), dtype=torch.float32, device=dev)
             count = torch.empty((nq,), dtype=torch.int32, device=dev)
             _ffi.check(_ffi.lib().cuddle_int4_search_device(C.byref(self._desc), q.data_ptr(), kind, nq, k, m, ids.data_ptr(), dist.data_ptr(),
-                                                            count.data_ptr(), ws.data_ptr(), need, index, st))
+                                                            count.data_ptr(), at, need, index, st))
         return ids, dist, count
 
     # ---- host forms, as ClusteredIndex has them ---------------------------------------------------
@@ -250,6 +254,6 @@ def rows_grad_device(grad_out: torch.Tensor, ids: torch.Tensor, n_rows: int, sca
         _ffi.check(_ffi.lib().cuddle_rows_grad_workspace(ids.numel(), n_rows, dim, C.byref(need)))
         ws = _workspace(need.value, dev)
         _ffi.check(_ffi.lib().cuddle_rows_grad_device(g.data_ptr(), kind, g.stride(0) if g.shape[0] > 1 else dim, ids.data_ptr(), bits, ids.numel(),
-                                                      float(scale), n_rows, dim, flags, out_kind, grad.data_ptr(), ws.data_ptr(), need.value,
+                                                      float(scale), n_rows, dim, flags, out_kind, grad.data_ptr(), None if ws is None else ws.data_ptr(), need.value,
                                                       index, st))
     return grad

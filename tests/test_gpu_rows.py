@@ -140,6 +140,23 @@ def test_distances_of_extreme_queries(gpu):
     assert (d >= 0).all() and np.all(np.abs(d - own) <= ref.distance_tolerance(values, values, own, "l2"))
 
 
+def test_distances_of_extreme_rows(gpu):
+    """Rows from 1e-36 to 1e36 against queries from 1e-9 to 1e9: products that f32 holds come out, others are infinite."""
+    rng = np.random.default_rng(12)
+    x = rng.standard_normal((73, 100)) * 10.0 ** np.linspace(-36, 36, 73)[:, None]
+    q = rng.standard_normal((7, 100)) * 10.0 ** np.linspace(-9, 9, 7)[:, None]
+    x, q = x.astype(np.float32), q.astype(np.float32)
+    for group in (32, 64, 128):
+        values = ref.encode(x, group)[2]
+        r = R.int4_encode_device(torch.from_numpy(x).cuda(gpu), group)
+        for metric in ("dot", "cosine", "l2"):
+            want = ref.distances(values, q, metric)
+            got = _np(r.distances_device(torch.from_numpy(q).cuda(gpu), metric))
+            fits = np.abs(want) < 3.4e38
+            tol = ref.distance_tolerance(values, q, want, metric)
+            assert np.all((np.abs(got - want) <= tol)[fits]) and np.isinf(got[np.abs(want) > 3.41e38]).all()
+
+
 def test_whole_numbers_are_exact(gpu):
     """SIFT-like rows whose groups all reach 7 * 2^j: scales are powers of two, every distance is a whole number."""
     rng = np.random.default_rng(2)
@@ -155,7 +172,8 @@ def test_whole_numbers_are_exact(gpu):
 # ---- search -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("n,d,nq,k,metric", [(1, 8, 2, 1, "l2"), (7, 64, 3, 10, "cosine"), (100, 32, 1, 100, "dot"), (8192, 64, 2, 10, "l2"),
                                              (8193, 64, 5, 1, "l2"), (20000, 48, 3, 1024, "cosine"), (100_000, 32, 2, 1000, "l2"), (70_000, 64, 9, 33, "dot"),
-                                             (16384, 16, 1, 7, "l2"), (3000, 130, 40, 64, "l2")])
+                                             (16384, 16, 1, 7, "l2"), (3000, 130, 40, 64, "l2"), (400_000, 16, 1, 200, "l2"), (50_000, 24, 1, 100, "cosine"),
+                                             (30_000, 8, 3, 16, "dot")])
 def test_search(gpu, n, d, nq, k, metric):
     x = torch.from_numpy(clustered(n, d, 30, n + d)).cuda(gpu)
     q = torch.from_numpy(clustered(nq, d, 30, n + d + 1) + 0.01).cuda(gpu)
@@ -344,6 +362,25 @@ def test_rows_grad_skewed_and_strided(gpu):
     assert not R.rows_grad_device(wide[:, :d], torch.full_like(ids, -7), n).any()
     same = R.rows_grad_device(wide[:, :d], torch.zeros_like(ids), n)
     _check_grad(same, wide[:, :d], torch.zeros_like(ids), n, 1.0, F32)
+
+
+def test_rows_grad_broadcast_and_shapes(gpu):
+    """One gradient row handed to every place (an expanded tensor), ids of two dimensions, a transposed gradient."""
+    dev = torch.device("cuda", gpu)
+    ids = torch.tensor([[3, 1, 3], [-1, 0, 3]], device=dev)
+    one = torch.arange(8, device=dev, dtype=F32)
+    want = torch.zeros((5, 8), device=dev)
+    want[3], want[1], want[0] = 3 * one, one, one
+    assert torch.equal(R.rows_grad_device(one.expand(2, 3, 8), ids, 5), want)
+    g = torch.randn((8, 6), device=dev)
+    got = R.rows_grad_device(g.t(), ids.reshape(-1), 5)
+    _check_grad(got, g.t(), ids.reshape(-1), 5, 1.0, F32)
+    with pytest.raises(ValueError):
+        R.rows_grad_device(one.expand(2, 2, 8), ids, 5)
+    with pytest.raises(ValueError):
+        R.rows_grad_device(one.expand(2, 3, 8), ids, 5, out=torch.zeros((5, 9), device=dev))
+    with pytest.raises(ValueError):
+        R.rows_grad_device(one.expand(2, 3, 8), ids.float(), 5)
 
 
 def test_gradient_against_differences(gpu):

@@ -2938,7 +2938,7 @@ RowShape row_shape(uint32_t pieces, uint64_t rows) {
     r.w = (pieces + parts - 1) / parts;
     r.rpi = 256 / r.w;
     r.rpb = rows * parts / r.rpi > 4096 ? r.rpi * 4 : r.rpi;
-    r.grid = dim3(grid_for((rows + r.rpb - 1) / r.rpb), parts);
+    r.grid = dim3((unsigned)std::min<uint64_t>((rows + r.rpb - 1) / r.rpb, (1u << 20) / parts), parts); // far from 2^32 threads
     return r;
 }
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -3351,7 +3351,7 @@ extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows,
         uint64_t stride = rows->n, items = rows->n;
         int level = 0;
         for (; items > kTopChunk; ++level) {
-            const uint32_t chunk = top_chunk(items, nq, k);
+            const uint32_t chunk = level == 0 ? top_chunk(items, nq, k) : kTopChunk; // the work space is laid out for these
             const uint64_t parts = (items + chunk - 1) / chunk;
             uint64_t *out = (uint64_t *)(ws + w.sel[level & 1]);
             auto go = [&](auto kernel) {

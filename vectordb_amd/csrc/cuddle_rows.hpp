@@ -409,17 +409,12 @@ __device__ __forceinline__ void int4_block_digits(const TQ *queries, uint32_t nq
     }
 }
 
-// The running sum of one (row, query) pair. The upper two digits' part in f64, the lower two's, 2^-16 of it, in f32:
-// its rounding is 2^-40 of the whole.
-struct Int4Sum {
-    double hi;
-    float lo;
-    __device__ __forceinline__ void add(i32x4_t c, float s) { // c: one group's integer products, digit by digit
-        lo = __builtin_fmaf(s, (float)(c[0] + (c[1] << 8)), lo);
-        hi = __builtin_fma((double)s, (double)(c[2] + (c[3] << 8)), hi);
-    }
-    __device__ __forceinline__ double value() const { return __builtin_fma(hi, 65536.0, (double)lo); }
-};
+// The running sum of one (row, query) pair gains one group: c = the integer products of the four digits, put together
+// exactly (42 bits), times the group's scale. In f64 throughout: an f32 part for the lower digits would overflow where rows
+// are large, and measured no faster (1M x 960, 64 queries: 476 us against 500).
+__device__ __forceinline__ double int4_add(double acc, i32x4_t c, double s) {
+    return __builtin_fma(s, __builtin_fma((double)(c[2] + (c[3] << 8)), 65536.0, (double)(c[0] + (c[1] << 8))), acc);
+}
 
 __host__ __device__ constexpr int int4_block(int qt) { return qt >= 3 ? 512 : 256; } // threads
 
@@ -452,12 +447,11 @@ struct Int4Held { uint32_t key, row, q; };
 
 // The candidates' pass asks of nearly every (row, query) pair only whether its distance is beyond the bound, and f32
 // answers that where it is not close. With S = the sum rounded to f32 a distance is t = A * S * R + B plus a constant of
-// the query: l2 A = -2 scale, B = |x|^2; dot A = -scale; cosine A = -scale / |q|, R = 1 / |x|. S is off by at most 2^-23
-// of itself and of its upper part, which differ by less than 2^-6 |x||q| / scale (the lower digits are at most 2^-13 of
-// the largest component, times sqrt(dim)). |S| scale <= |x||q|, at most (|x|^2 + |q|^2) / 2: for l2 all roundings together
-// stay below 2^-20 (|x|^2 + |q|^2), for cosine below 2^-20, taken off B and added to C = bound - constant beforehand.
-// dot has no such measure at hand: S is moved by 2^-20 of itself and its lower part. t > C: surely beyond. What is not a
-// number, or too large or small for f32, is not "beyond" and goes on to the exact evaluation.
+// the query: l2 A = -2 scale, B = |x|^2; dot A = -scale; cosine A = -scale / |q|, R = 1 / |x|. |S| scale <= |x||q|, at most
+// (|x|^2 + |q|^2) / 2, and each of fewer than eight roundings is at most 2^-24 of one of the terms: for l2 they stay below
+// 2^-20 (|x|^2 + |q|^2), for cosine below 2^-20, taken off B and added to C = bound - constant beforehand, twice over.
+// dot has no such measure at hand: S is moved by 2^-20 of itself. t > C: surely beyond. What is not a number, or too
+// large or small for f32, is not "beyond" and goes on to the exact evaluation.
 struct Int4Test {
     float A, C;
 };
@@ -478,11 +472,11 @@ __device__ __forceinline__ float int4_test_row(uint32_t metric, double xsq) {
     return metric == kMetricCosine ? (float)inv_sqrt(xsq) : (float)(xsq * (1.0 - 1.0 / (1 << 19)));
 }
 template <uint32_t METRIC>
-__device__ __forceinline__ bool int4_beyond(double hi, float lo, const Int4Test &q, float row) {
-    float S = __builtin_fmaf((float)hi, 65536.f, lo);
+__device__ __forceinline__ bool int4_beyond(double sum, const Int4Test &q, float row) {
+    float S = (float)sum;
     if (METRIC == kMetricL2) return __builtin_fmaf(q.A, S, row) > q.C;
     if (METRIC == kMetricCosine) return q.A * (S * row) > q.C;
-    S = __builtin_fmaf(fabsf(lo) + fabsf(S), 0x1p-20f, S); // A < 0: a larger S is a smaller t
+    S = __builtin_fmaf(fabsf(S), 0x1p-20f, S); // A < 0: a larger S is a smaller t
     const float t = q.A * S;
     return t > q.C && t < 3.0e38f;
 }
@@ -617,11 +611,11 @@ int4_distance_kernel(Int4DistArgs a) {
             row[t] = (a.stride ? int4_sampled(i, a.stride) : i) * 16 + r;
             xsq[t] = a.metric == kMetricDot ? 0.0 : a.sqnorm[min(row[t], a.n - 1)];
         }
-        Int4Sum acc[T][QT];
+        double acc[T][QT];
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
-            for (int q = 0; q < QT; ++q) acc[t][q] = Int4Sum{0.0, 0.f};
+            for (int q = 0; q < QT; ++q) acc[t][q] = 0.0;
         for (uint32_t u0 = 0; u0 < a.units; u0 += a.ku) {
             if (!FUSED && a.units > a.ku) {
                 __syncthreads();
@@ -658,14 +652,14 @@ int4_distance_kernel(Int4DistArgs a) {
                             const uint2 v = w[t][p0 + p];
                             b[p] = i32x4_t{(int)((v.x << 4) & M), (int)((v.y << 4) & M), (int)(v.x & M), (int)(v.y & M)};
                         }
-                        auto scale = [&](int i) { return bf16_to_f32(sc[t].v[i]); };
+                        auto scale = [&](int i) { return (double)bf16_to_f32(sc[t].v[i]); };
                         if (G == 32) {
                             auto half = [](i32x4_t v, int i) { return (long)(uint32_t)v[2 * i] | (long)((uint64_t)(uint32_t)v[2 * i + 1] << 32); };
 #pragma unroll
                             for (int i = 0; i < 2; ++i)
 #pragma unroll
                                 for (int q = 0; q < QT; ++q)
-                                    acc[t][q].add(__builtin_amdgcn_mfma_i32_16x16x32_i8(half(dg[0][q], i), half(b[0], i), zero, 0, 0, 0), scale(2 * p0 + i));
+                                    acc[t][q] = int4_add(acc[t][q], __builtin_amdgcn_mfma_i32_16x16x32_i8(half(dg[0][q], i), half(b[0], i), zero, 0, 0, 0), scale(2 * p0 + i));
                         } else {
                             i32x4_t c[QT];
 #pragma unroll
@@ -675,7 +669,7 @@ int4_distance_kernel(Int4DistArgs a) {
                                 for (int q = 0; q < QT; ++q) c[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(dg[PP - 1][q], b[PP - 1], c[q], 0, 0, 0);
                             }
 #pragma unroll
-                            for (int q = 0; q < QT; ++q) acc[t][q].add(c[q], scale(p0 / PP));
+                            for (int q = 0; q < QT; ++q) acc[t][q] = int4_add(acc[t][q], c[q], scale(p0 / PP));
                         }
                     }
                 }
@@ -691,15 +685,15 @@ int4_distance_kernel(Int4DistArgs a) {
                     constexpr uint32_t M = decltype(metric)::value;
                     uint64_t any = 0;
 #pragma unroll
-                    for (int q = 0; q < QT; ++q) any |= __ballot(!int4_beyond<M>(acc[t][q].hi, acc[t][q].lo, s_test[q * 4 + h], rt));
+                    for (int q = 0; q < QT; ++q) any |= __ballot(!int4_beyond<M>(acc[t][q], s_test[q * 4 + h], rt));
                     if (!any) return;
 #pragma unroll
                     for (int q = 0; q < QT; ++q) {
-                        const bool take = real && !int4_beyond<M>(acc[t][q].hi, acc[t][q].lo, s_test[q * 4 + h], rt);
+                        const bool take = real && !int4_beyond<M>(acc[t][q], s_test[q * 4 + h], rt);
                         if (!__ballot(take)) continue;
                         const uint32_t qi = (y * QT + q) * 4 + h;
                         const Int4Query qv = s_info[q * 4 + h];
-                        const uint32_t key = f32_key(int4_finish(M, acc[t][q].value(), qv.scale, xsq[t], qv.sq));
+                        const uint32_t key = f32_key(int4_finish(M, acc[t][q], qv.scale, xsq[t], qv.sq));
                         keep(take && qi < a.nq && key <= s_tau[q * 4 + h], key, (uint32_t)row[t], qi);
                     }
                 };
@@ -714,7 +708,7 @@ int4_distance_kernel(Int4DistArgs a) {
                 const uint32_t q0 = (y * QT + q) * 4;
                 const Int4Query qv = s_info[q * 4 + h];
                 float *o = a.dist + q0 * a.dstride + i * 16;
-                const float d = int4_finish(a.metric, acc[t][q].value(), qv.scale, xsq[t], qv.sq);
+                const float d = int4_finish(a.metric, acc[t][q], qv.scale, xsq[t], qv.sq);
                 if (q0 + h < a.nq) o[out_at] = row[t] < a.n ? d : __builtin_nanf(""); // NaN sorts last: never makes the bound smaller
             }
         }

@@ -3355,7 +3355,8 @@ extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows,
             const uint64_t parts = (items + chunk - 1) / chunk;
             uint64_t *out = (uint64_t *)(ws + w.sel[level & 1]);
             auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)parts, nq), dim3(kTopThreads), 0, s, in, stride, items, k, chunk, out, (const uint32_t *)cnt, kTopChunk);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)(cnt ? std::min<uint64_t>(parts, 8) : parts), nq), dim3(kTopThreads), 0, s, in, stride, items, k, chunk,
+                                   (uint32_t)parts, out, (const uint32_t *)cnt, kTopChunk);
             };
             if (level == 0) go(int4_topk_level_kernel<true>);
             else go(int4_topk_level_kernel<false>);

@@ -353,57 +353,73 @@ __device__ __forceinline__ float int4_finish(uint32_t metric, double sum, double
     return d < 0.f ? 0.f : d; // the three terms of a row next to the query round apart
 }
 
-// The digits of the queries [4 * w] .. of one quartet, made by a block of 256 threads straight into LDS (wave w takes
-// query q0 + w): what int4_query_kernel writes, for blocks that need a single quartet and hold all of it. Units from
-// ceil(dim / 64) to `pad` are zero.
+// The digits of one quartet of queries, made by a block of 256 threads straight into LDS: what int4_query_kernel writes,
+// for blocks that need a single quartet and hold all of it. Every wave has a quarter of the units of every query, so that
+// a lone query is read in one trip. Units from ceil(dim / 64) to `pad` and queries from nq on are zero.
 template <class TQ>
 __device__ __forceinline__ void int4_block_digits(const TQ *queries, uint32_t nq, uint32_t dim, uint32_t pad, uint8_t *dig, Int4Query *info) {
-    const uint32_t q = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const bool real = q < nq;
-    const TQ *src = queries + (uint64_t)(real ? q : 0) * dim;
-    float m = 0.f;
-    double sq = 0.0;
+    __shared__ float s_max[4][4];
+    __shared__ double s_sq[4][4];
+    const uint32_t w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     constexpr int U = 8; // units read at a time
-    auto read8 = [&](uint32_t u0, float (&v)[U]) {
+    auto read8 = [&](const TQ *src, uint32_t u0, float (&v)[U]) {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const uint32_t i = (u0 + j) * 64 + lane;
-            v[j] = real && i < dim ? to_f32(src[min(i, dim - 1)]) : 0.f;
+            const uint32_t i = (u0 + 4 * j) * 64 + lane;
+            v[j] = i < dim ? to_f32(src[i]) : 0.f;
         }
     };
-    for (uint32_t u0 = 0; u0 * 64 < dim; u0 += U) {
-        float v[U];
-        read8(u0, v);
+    for (uint32_t q = 0; q < nq; ++q) {
+        float m = 0.f;
+        double sq = 0.0;
+        for (uint32_t u0 = w; u0 * 64 < dim; u0 += 4 * U) {
+            float v[U];
+            read8(queries + (uint64_t)q * dim, u0, v);
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const float a = fabsf(v[j]);
-            m = fmaxf(m, a <= 3.4028234663852886e38f ? a : __builtin_huge_valf());
-            sq = __builtin_fma((double)v[j], (double)v[j], sq);
+            for (int j = 0; j < U; ++j) {
+                const float a = fabsf(v[j]);
+                m = fmaxf(m, a <= 3.4028234663852886e38f ? a : __builtin_huge_valf());
+                sq = __builtin_fma((double)v[j], (double)v[j], sq);
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            m = fmaxf(m, __shfl_xor(m, d, 64));
+            sq += __shfl_xor(sq, d, 64);
+        }
+        if (lane == 0) {
+            s_max[q][w] = m;
+            s_sq[q][w] = sq;
         }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        m = fmaxf(m, __shfl_xor(m, d, 64));
-        sq += __shfl_xor(sq, d, 64);
-    }
-    const bool bad = m > 3.4028234663852886e38f;
-    int e = 0;
-    if (!bad && m > 0.f) (void)frexp((double)m, &e);
-    const double up = ldexp(1.0, 30 - e);
-    if (lane == 0) info[q] = Int4Query{bad ? __builtin_nan("") : ldexp(1.0, e - 34), sq};
+    __syncthreads();
     const uint32_t h = (lane & 31) >> 3, b = ((lane >> 5) << 3) | (lane & 7); // the lane's component of every unit
-    for (uint32_t u0 = 0; u0 < pad; u0 += U) {
-        float v[U];
-        read8(u0, v);
+    for (uint32_t q = 0; q < 4; ++q) {
+        const bool real = q < nq;
+        const float m = real ? fmaxf(fmaxf(s_max[q][0], s_max[q][1]), fmaxf(s_max[q][2], s_max[q][3])) : 0.f;
+        const bool bad = m > 3.4028234663852886e38f;
+        int e = 0;
+        if (!bad && m > 0.f) (void)frexp((double)m, &e);
+        const double up = ldexp(1.0, 30 - e);
+        if (threadIdx.x == 0)
+            info[q] = Int4Query{bad ? __builtin_nan("") : ldexp(1.0, e - 34), real ? (s_sq[q][0] + s_sq[q][1]) + (s_sq[q][2] + s_sq[q][3]) : 0.0};
+        for (uint32_t u0 = w; u0 < pad; u0 += 4 * U) {
+            float v[U];
+            if (real)
+                read8(queries + (uint64_t)q * dim, u0, v);
+            else
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            if (u0 + j >= pad) break;
-            int32_t f = (int32_t)rint((double)(bad ? 0.f : v[j]) * up);
+                for (int j = 0; j < U; ++j) v[j] = 0.f;
 #pragma unroll
-            for (uint32_t d = 0; d < 4; ++d) {
-                const int32_t lo = (int32_t)(int8_t)(f & 255);
-                f = (f - lo) >> 8;
-                dig[(u0 + j) * 1024 + ((h << 4) | (q << 2) | d) * 16 + b] = (uint8_t)lo;
+            for (int j = 0; j < U; ++j) {
+                if (u0 + 4 * j >= pad) break;
+                int32_t f = (int32_t)rint((double)(bad ? 0.f : v[j]) * up);
+#pragma unroll
+                for (uint32_t d = 0; d < 4; ++d) {
+                    const int32_t lo = (int32_t)(int8_t)(f & 255);
+                    f = (f - lo) >> 8;
+                    dig[(u0 + 4 * j) * 1024 + ((h << 4) | (q << 2) | d) * 16 + b] = (uint8_t)lo;
+                }
             }
         }
     }
@@ -719,21 +735,20 @@ int4_distance_kernel(Int4DistArgs a) {
 // ---------------------------------------------------------------------------------------------
 // top-k of rows of distances
 // ---------------------------------------------------------------------------------------------
-// A selection is a list of (key << 32 | row) in row order; keys are f32_key (NaN after everything). A level cuts a
-// query's items into chunks and keeps each chunk's k smallest keys, equal keys by position; chunks are in row order and
-// only the last can be short of k, so positions stay the order of the rows and the padding (~0) stays at the end.
+// An item is (key << 32 | row); keys are f32_key (NaN after everything), equal keys go by row. A level cuts a query's
+// items into chunks and keeps each chunk's k smallest, in any order; a chunk short of k is filled up with ~0, which
+// stands behind every row.
 // Many rows and queries: the distances are not written at all. The k-th smallest key of a sample of the rows bounds the
 // k-th smallest of all, a pass over the rows collects those within the bound (a few thousand), and the k smallest of the
 // collection are the answer. Where the collection overflows, the levels answer instead.
 constexpr uint32_t kTopChunk = 8192;
 constexpr uint32_t kTopMaxK = 1024;
-constexpr uint32_t kTopThreads = 512;
+constexpr uint32_t kTopThreads = 1024;
 
 struct TopkLds {
     uint32_t hist[256];
     uint32_t lo[kTopThreads / 64], hi[kTopThreads / 64];
-    uint32_t bin, rest, full;
-    uint32_t wtmp[2 * kTopThreads / 64];
+    uint32_t bin, rest, full, n;
 };
 
 // T and budget such that the k smallest (1 <= k <= C) of the keys key(0) .. key(C - 1) are those below T and `budget` of
@@ -804,29 +819,60 @@ __device__ __forceinline__ void block_kth_key(uint32_t C, uint32_t k, KeyFn key,
     T = prefix;
 }
 
+// The k smallest of C items with keys keys[i] (LDS) and item(i) = key << 32 | row: emit(place, item) in any order, places
+// 0 .. min(k, C) - 1. Of the items equal to the last key the lowest rows. s.n is zero on entry. All threads of the block.
+template <class ItemFn, class EmitFn>
+__device__ __forceinline__ void block_smallest(const uint32_t *keys, uint32_t C, uint32_t k, ItemFn item, EmitFn emit, TopkLds &s) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t T = 0xFFFFFFFFu, budget = C, R = 0xFFFFFFFFu, rest;
+    if (C > k) {
+        block_kth_key(C, k, [&](uint32_t i) { return keys[i]; }, s, T, budget);
+        if (budget < C) { // T is a key of its own: are there more items with it than wanted?
+            uint32_t ties = 0;
+            for (uint32_t i = tid; i < C; i += kTopThreads) ties += keys[i] == T ? 1u : 0u;
+            if (ties) atomicAdd(&s.n, ties);
+            __syncthreads();
+            ties = s.n;
+            __syncthreads();
+            if (tid == 0) s.n = 0;
+            if (ties > budget) block_kth_key(C, budget, [&](uint32_t i) { return keys[i] == T ? (uint32_t)item(i) : 0xFFFFFFFFu; }, s, R, rest);
+            __syncthreads();
+        }
+    }
+    for (uint32_t i = tid; i < C; i += kTopThreads) {
+        if (keys[i] > T) continue;
+        const uint64_t v = item(i);
+        if (keys[i] < T || (uint32_t)v <= R) emit(atomicAdd(&s.n, 1u), v);
+    }
+}
+
 // Level: from f32 distances (FIRST) or from the previous level's lists. in: [nq][in_stride]; out: [nq][parts][k].
-// chunk <= kTopChunk items per block. redo: nullptr, or only queries that count more than `cap`. grid (parts, nq), block
-// kTopThreads.
+// chunk <= kTopChunk items at a time. redo: nullptr, or only queries that count more than `cap` (few blocks then, since
+// hardly ever one has work). grid (at most parts, nq), block kTopThreads.
 template <bool FIRST>
 __global__ void __launch_bounds__(kTopThreads)
-int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint32_t k, uint32_t chunk, uint64_t *out, const uint32_t *redo, uint32_t cap) {
+int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint32_t k, uint32_t chunk, uint32_t parts, uint64_t *out, const uint32_t *redo,
+                       uint32_t cap) {
     __shared__ uint32_t keys[kTopChunk];
     __shared__ TopkLds s;
     if (redo && redo[blockIdx.y] <= cap) return;
-    const uint64_t base = (uint64_t)blockIdx.x * chunk;
-    const uint32_t C = (uint32_t)min((uint64_t)chunk, items - base), tid = threadIdx.x;
-    const float *df = static_cast<const float *>(in) + (uint64_t)blockIdx.y * in_stride + base;
-    const uint64_t *dl = static_cast<const uint64_t *>(in) + (uint64_t)blockIdx.y * in_stride + base;
+    const uint32_t tid = threadIdx.x;
+    for (uint32_t part = blockIdx.x; part < parts; part += gridDim.x) {
+        const uint64_t base = (uint64_t)part * chunk;
+        const uint32_t C = (uint32_t)min((uint64_t)chunk, items - base);
+        const float *df = static_cast<const float *>(in) + (uint64_t)blockIdx.y * in_stride + base;
+        const uint64_t *dl = static_cast<const uint64_t *>(in) + (uint64_t)blockIdx.y * in_stride + base;
+        __syncthreads(); // the part before has been read
 #pragma unroll 8
-    for (uint32_t i = tid; i < C; i += kTopThreads) keys[i] = FIRST ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
-    __syncthreads();
-    uint64_t *o = out + ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * k;
-    uint32_t T = 0xFFFFFFFFu, budget = C;
-    if (C > k) block_kth_key(C, k, [&](uint32_t i) { return keys[i]; }, s, T, budget);
-    ordered_threshold_compact(
-        C, T, budget, [&](uint32_t i) -> uint32_t { return keys[i]; },
-        [&](uint32_t i, uint32_t kv, uint32_t rank) { o[rank] = FIRST ? ((uint64_t)kv << 32 | (uint32_t)(base + i)) : dl[i]; }, s.wtmp);
-    for (uint32_t i = C + tid; i < k; i += kTopThreads) o[i] = ~0ull;
+        for (uint32_t i = tid; i < C; i += kTopThreads) keys[i] = FIRST ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        uint64_t *o = out + ((uint64_t)blockIdx.y * parts + part) * k;
+        block_smallest(
+            keys, C, k, [&](uint32_t i) -> uint64_t { return FIRST ? (uint64_t)keys[i] << 32 | (uint32_t)(base + i) : dl[i]; },
+            [&](uint32_t at, uint64_t v) { o[at] = v; }, s);
+        for (uint32_t i = C + tid; i < k; i += kTopThreads) o[i] = ~0ull;
+    }
 }
 
 // The bound of a query: the k-th smallest key of its sample, and its candidate count set to zero. One block per query;
@@ -864,7 +910,6 @@ int4_topk_final_kernel(const void *in, uint64_t in_stride, uint32_t items, uint3
     __shared__ uint32_t keys[kTopChunk];
     __shared__ uint64_t sel[kTopMaxK];
     __shared__ TopkLds s;
-    __shared__ uint32_t s_n;
     const uint32_t tid = threadIdx.x, q = blockIdx.x;
     if (KIND == 2) {
         items = cnt[q];
@@ -877,32 +922,11 @@ int4_topk_final_kernel(const void *in, uint64_t in_stride, uint32_t items, uint3
     for (uint32_t i = tid; i < items; i += kTopThreads) keys[i] = KIND == 0 ? f32_key(df[i]) : (uint32_t)(dl[i] >> 32);
     const uint32_t width = next_pow2(min(k, items));
     for (uint32_t i = tid; i < width; i += kTopThreads) sel[i] = ~0ull;
-    if (tid == 0) s_n = 0;
+    if (tid == 0) s.n = 0;
     __syncthreads();
-    uint32_t T = 0xFFFFFFFFu, budget = items;
-    if (items > k) block_kth_key(items, k, [&](uint32_t i) { return keys[i]; }, s, T, budget);
-    if (KIND == 2) {
-        // of the candidates equal to the k-th key the `budget` lowest rows: the budget-th smallest row among them
-        uint32_t R = 0xFFFFFFFFu, rest;
-        if (items > k) {
-            uint32_t ties = 0;
-            for (uint32_t i = tid; i < items; i += kTopThreads) ties += keys[i] == T ? 1u : 0u;
-            if (ties) atomicAdd(&s_n, ties);
-            __syncthreads();
-            ties = s_n;
-            __syncthreads();
-            if (tid == 0) s_n = 0;
-            if (ties > budget) block_kth_key(items, budget, [&](uint32_t i) { return keys[i] == T ? (uint32_t)dl[i] : 0xFFFFFFFFu; }, s, R, rest);
-            __syncthreads();
-        }
-        for (uint32_t i = tid; i < items; i += kTopThreads) {
-            const uint64_t v = keys[i] <= T ? dl[i] : ~0ull;
-            if (keys[i] < T || (keys[i] == T && (uint32_t)v <= R)) sel[atomicAdd(&s_n, 1u)] = v;
-        }
-    } else
-        ordered_threshold_compact(
-            items, T, budget, [&](uint32_t i) -> uint32_t { return keys[i]; },
-            [&](uint32_t i, uint32_t kv, uint32_t rank) { sel[rank] = KIND == 0 ? ((uint64_t)kv << 32 | i) : dl[i]; }, s.wtmp);
+    block_smallest(
+        keys, items, k, [&](uint32_t i) -> uint64_t { return KIND == 0 ? (uint64_t)keys[i] << 32 | i : dl[i]; },
+        [&](uint32_t at, uint64_t v) { sel[at] = v; }, s);
     __syncthreads();
     block_sort_u64(sel, width);
     for (uint32_t i = tid; i < k; i += kTopThreads) {

@@ -55,16 +55,19 @@ def _id_bits(ids: torch.Tensor) -> int:
     return 32 if ids.dtype == torch.int32 else 64
 
 
+_NO_CTX = contextlib.nullcontext()
+
+
 def _enter(dev: torch.device, stream, *inputs: torch.Tensor):
     """(context, device index, hipStream_t) for work on `dev` and `stream`: inside the context torch's copies and
     allocations belong to the stream. Inputs used on a stream that is not the current one are kept for it."""
     index = dev.index if dev.index is not None else torch.cuda.current_device()
-    cur = torch.cuda.current_stream(dev)
+    cur = torch.cuda.current_stream(index)
     if stream is None or stream == cur:
-        return contextlib.nullcontext(), index, C.c_void_p(cur.cuda_stream)
+        return _NO_CTX, index, cur.cuda_stream
     for t in inputs:
         t.record_stream(stream)
-    return torch.cuda.stream(stream), index, C.c_void_p(stream.cuda_stream)
+    return torch.cuda.stream(stream), index, stream.cuda_stream
 
 
 def _workspace(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:

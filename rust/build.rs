@@ -11,7 +11,9 @@ fn main() {
         .args([
             "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
             // distances reproduce the NEON accumulation order bit for bit: no contraction, correctly rounded division
-            "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-fast-math", "-o",
+            "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-fast-math",
+            // no packed f32 instructions
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-o",
         ])
         .arg(out.join("libcuddle_hip.so"))
         .arg(format!("{src}/cuddle_hip.hip"))

@@ -55,6 +55,16 @@ pub struct CuddleStats {
     pub rabitq_exact_all_queries: u64,
 }
 
+#[repr(C)]
+pub struct CuddleInt4Rows {
+    pub codes: *mut c_void,
+    pub scales: *mut c_void,
+    pub sqnorm: *mut c_void,
+    pub n: u64,
+    pub dim: u32,
+    pub group: u32,
+}
+
 extern "C" {
     pub fn cuddle_abi_version() -> u32;
     pub fn cuddle_last_error() -> *const c_char;
@@ -90,6 +100,36 @@ extern "C" {
     pub fn cuddle_kmeans_assign(
         d_vectors: *const f32, n: u64, d_centroids: *const f32, k: u32, dim: u32, metric: u32, d_assign: *mut u32,
         d_dist: *mut f32, out_fallbacks: *mut u64, device_id: c_int, stream: *mut c_void,
+    ) -> c_int;
+    // embedding table: 4-bit rows, row lookup, its gradient (device pointers, enqueued on `stream`)
+    pub fn cuddle_int4_sizes(n: u64, dim: u32, group: u32, code_bytes: *mut u64, scale_stride: *mut u32) -> c_int;
+    pub fn cuddle_int4_encode_device(
+        rows: *const CuddleInt4Rows, first_row: u64, count: u64, d_vectors: *const c_void, ty: u32, row_stride: u64,
+        device_id: c_int, stream: *mut c_void,
+    ) -> c_int;
+    pub fn cuddle_int4_lookup_device(
+        rows: *const CuddleInt4Rows, d_ids: *const c_void, id_bits: u32, n_ids: u64, scale: f32, out_type: u32,
+        d_out: *mut c_void, device_id: c_int, stream: *mut c_void,
+    ) -> c_int;
+    pub fn cuddle_int4_workspace(n: u64, dim: u32, n_queries: u32, k: u32, bytes: *mut u64) -> c_int;
+    pub fn cuddle_int4_distances_device(
+        rows: *const CuddleInt4Rows, d_queries: *const c_void, ty: u32, n_queries: u32, metric: u32, d_dist: *mut f32,
+        d_ws: *mut c_void, ws_bytes: u64, device_id: c_int, stream: *mut c_void,
+    ) -> c_int;
+    pub fn cuddle_int4_search_device(
+        rows: *const CuddleInt4Rows, d_queries: *const c_void, ty: u32, n_queries: u32, k: u32, metric: u32,
+        d_out_ids: *mut u64, d_out_dist: *mut f32, d_out_count: *mut u32, d_ws: *mut c_void, ws_bytes: u64,
+        device_id: c_int, stream: *mut c_void,
+    ) -> c_int;
+    pub fn cuddle_rows_lookup_device(
+        d_table: *const c_void, ty: u32, row_stride: u64, n_rows: u64, dim: u32, d_ids: *const c_void, id_bits: u32,
+        n_ids: u64, scale: f32, d_out: *mut c_void, device_id: c_int, stream: *mut c_void,
+    ) -> c_int;
+    pub fn cuddle_rows_grad_workspace(n_ids: u64, n_rows: u64, dim: u32, bytes: *mut u64) -> c_int;
+    pub fn cuddle_rows_grad_device(
+        d_grad_out: *const c_void, ty: u32, row_stride: u64, d_ids: *const c_void, id_bits: u32, n_ids: u64, scale: f32,
+        n_rows: u64, dim: u32, flags: u32, grad_type: u32, d_grad: *mut c_void, d_ws: *mut c_void, ws_bytes: u64,
+        device_id: c_int, stream: *mut c_void,
     ) -> c_int;
     // one process per GPU: RCCL communicator + the exact sharded search
     pub fn cuddle_comm_unique_id(id: *mut u8) -> c_int;

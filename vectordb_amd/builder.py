@@ -196,6 +196,15 @@ def _kmeans_fit_native(x: torch.Tensor, k: int, metric: int, max_iterations: int
     return cent, assign.long()
 
 
+def _take(x: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
+    """Rows of x by index; on the GPU through the library (rows_lookup_device: the same values)."""
+    if not x.is_cuda:
+        return x[idx]
+    from .rows import rows_lookup_device
+
+    return rows_lookup_device(x, idx)
+
+
 class _Tree:
     def __init__(self):
         self.centroid: List[torch.Tensor] = []
@@ -216,10 +225,10 @@ def _build_recursive(tree: _Tree, x: torch.Tensor, idx: torch.Tensor, depth: int
     if n == 0:
         return []
     if n <= 2 * target_leaf or depth >= 10:  # :210
-        sub = x[idx]
+        sub = _take(x, idx)
         return [tree.add(sub.sum(0) / n, [], idx)]  # leaf centroid = mean (:509-531)
     k = min(max(math.ceil(n / target_leaf), 2), branching, n)  # :221-225
-    sub = x[idx]
+    sub = _take(x, idx)
     cent, assign = kmeans_fit(sub, k, metric, max_iterations, gen)
     clusters = []
     for c in range(k):
@@ -339,7 +348,8 @@ def build_index(vectors, branching_factor: int = 100, target_leaf_size: int = 10
         if cnt:
             order.append(tree.vec[i])
     ids_t = torch.cat(order) if order else torch.zeros(0, dtype=torch.long, device=dev)
-    vec_lc = x[ids_t].cpu().numpy()
+    stored = _take(x, ids_t)
+    vec_lc = stored.cpu().numpy()
     fi = FlatIndex(
         dim=d, metric=m, code_kind=_ffi.CODE_BINARY if code_kind == "binary" else _ffi.CODE_RABITQ,
         centroids=centroids, child_offsets=child_offsets, children=np.asarray(children, dtype=np.uint32),
@@ -361,17 +371,17 @@ def build_index(vectors, branching_factor: int = 100, target_leaf_size: int = 10
         else:
             fi.threshold = float(threshold)
         if dev.type == "cuda":
-            fi.codes = binary_encode_device(x[ids_t], fi.threshold).cpu().numpy().view(np.uint64)
+            fi.codes = binary_encode_device(stored, fi.threshold).cpu().numpy().view(np.uint64)
         else:
             fi.codes = pack_binary_codes(vec_lc, fi.threshold)
     elif code_kind == "rabitq":
         rot = make_rotation(d, seed + 7919)
         fi.rabitq_rot_t = rot
         if dev.type == "cuda":
-            c, nr, ip = rabitq_encode_device(x[ids_t], torch.from_numpy(rot).to(dev))
+            c, nr, ip = rabitq_encode_device(stored, torch.from_numpy(rot).to(dev))
             fi.rabitq_codes, fi.rabitq_norm, fi.rabitq_ip_oo = c.cpu().numpy().view(np.uint32), nr.cpu().numpy(), ip.cpu().numpy()
         else:
-            fi.rabitq_codes, fi.rabitq_norm, fi.rabitq_ip_oo = rabitq_encode(x[ids_t], torch.from_numpy(rot))
+            fi.rabitq_codes, fi.rabitq_norm, fi.rabitq_ip_oo = rabitq_encode(stored, torch.from_numpy(rot))
     else:
         raise ValueError(f"unknown code_kind {code_kind!r}")
     return fi.normalised()

@@ -161,7 +161,7 @@ __device__ __forceinline__ void rabitq_stage_query(const float *rq, uint32_t dim
 //   * tau = the rerank_k-th smallest upper bound est~ + E: at least rerank_k candidates have their exact
 //     estimate <= tau, so a candidate whose lower bound est~ - E is > tau cannot be selected;
 //   * the others (the selection and a band around its boundary) get the exact sequential-order
-//     estimate, two candidates per lane in packed f32 adds, and the selection runs on those values:
+//     estimate, two candidates per lane in the halves of a pair of floats, and the selection runs on those values:
 //     the same set, order and keys as evaluating every candidate exactly.
 // Bits of the quantised magnitudes. The scan's cost grows with every plane (two operations per code word and
 // plane); the error bound halves with every plane, and below ten the band of candidates that need the exact
@@ -211,7 +211,8 @@ __device__ __forceinline__ float rabitq_signed(uint32_t x, float mag) {
 }
 
 // compute_inner_product_fast (rabitq.rs:298-321) for TWO vectors at once: the sequential sums of both run
-// in the two halves of packed f32 adds (each half the same IEEE addition as the scalar sum), the sign of
+// in the two halves of a pair of floats (each half the same IEEE addition as the scalar sum; the build leaves
+// packed f32 instructions out, so these are two additions), the sign of
 // a term comes from bit 31 of the bit-reversed (query sign ^ ~code) word, which a 64-bit shift moves on
 // for both vectors in one instruction. ca / cb: the vectors' code columns (word w at ca[w * na]).
 __device__ __forceinline__ void rabitq_ip_pair(const uint32_t *ca, uint32_t na, const uint32_t *cb, uint32_t nb, uint32_t dim,

@@ -963,8 +963,8 @@ route_dist_grouped_kernel(IndexDev ix, const float *queries, const uint32_t *lev
 #pragma unroll
             for (uint32_t jh = 0; jh < kGroupNQ; jh += 4) { // four queries at a time
                 __builtin_amdgcn_sched_barrier(0);
-                // two-float vector arithmetic = the packed f32 instructions; each component is the
-                // same IEEE operation as the scalar form
+                // two-float vectors: each component is the same IEEE operation as the scalar form (and, packed f32
+                // instructions being left out of the build, one instruction of its own)
                 v2f acc_lo[4], acc_hi[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc_lo[j] = acc_hi[j] = v2f{0.f, 0.f};

@@ -901,6 +901,21 @@ __device__ __forceinline__ float f32_of_key(uint32_t k) { // NaN for the NaN's k
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+// Sort of n (a power of two, at most kTopThreads) distinct items, padded at the end with ~0: every item's place is the
+// number of items below it, counted by kTopThreads / n neighbouring lanes (64 at most), a part of the items each.
+__device__ __forceinline__ void block_sort_small(uint64_t *s, uint32_t n) {
+    const uint32_t per = min(64u, kTopThreads / n), i = threadIdx.x / per, part = threadIdx.x % per, m = max(1u, n / per);
+    const uint64_t v = i < n ? s[i] : ~0ull;
+    uint32_t place = 0;
+    if (i < n && part * m < n)
+#pragma unroll 8
+        for (uint32_t j = part * m; j < part * m + m; ++j) place += s[j] < v ? 1u : 0u;
+    for (uint32_t d = 1; d < per; d <<= 1) place += (uint32_t)__shfl_xor((int)place, (int)d, 64);
+    __syncthreads(); // every item has been read
+    if (part == 0 && i < n && v != ~0ull) s[place] = v;
+    __syncthreads();
+}
+
 // Last level: at most kTopChunk items; the k smallest, in order, as ids and distances. KIND 0: distances in row order,
 // 1: a level's list, 2: a collection in any order, count[q] of them (left alone where they overflowed).
 template <int KIND>
@@ -928,7 +943,7 @@ int4_topk_final_kernel(const void *in, uint64_t in_stride, uint32_t items, uint3
         keys, items, k, [&](uint32_t i) -> uint64_t { return KIND == 0 ? (uint64_t)keys[i] << 32 | i : dl[i]; },
         [&](uint32_t at, uint64_t v) { sel[at] = v; }, s);
     __syncthreads();
-    block_sort_u64(sel, width);
+    block_sort_small(sel, width);
     for (uint32_t i = tid; i < k; i += kTopThreads) {
         const bool have = i < found;
         ids[(uint64_t)q * k + i] = have ? (uint64_t)(uint32_t)sel[i] : ~0ull;

@@ -534,10 +534,12 @@ typedef enum cuddle_type { CUDDLE_TYPE_F32 = 0, CUDDLE_TYPE_F16 = 1, CUDDLE_TYPE
  * s = bf16(max|x| / 7), code c = rint(x / s) with halves to even, clamped to -7..7 (0 where s is 0); the
  * row stands for s * c. A group with a NaN or an infinity has s = NaN and codes 0: such a row decodes to
  * NaN there, and its distances are NaN.
- *   codes  : blocks of 16 rows x 64 components, 512 bytes each, the blocks of 16 rows one after the
- *            other; in a block row r has 32 bytes, byte 8h + i (h < 4, i < 8) holding component 8h + i in
- *            its low and 32 + 8h + i in its high nibble, two's complement; components past dim are 0, rows
- *            past n arbitrary. cuddle_int4_sizes gives the bytes. 16-byte aligned.
+ *   codes  : tiles of 16 rows, one after the other, U = ceil(dim / 64) units of 512 bytes each. A unit holds 64
+ *            components of 16 rows; (h < 4, i < 8) names the byte with component 8h + i in its low and
+ *            32 + 8h + i in its high nibble, two's complement. It is byte 64 r + 16 h + 8 (u & 1) + i of the
+ *            1024 bytes of units u & ~1 and u | 1, or, of an odd last unit, byte 32 r + 8 h + i of its 512.
+ *            Components past dim are 0, rows past n arbitrary. cuddle_int4_sizes gives the bytes (for odd U 16
+ *            more than that, of any value). 16-byte aligned.
  *   scales : [n][scale_stride] bf16, scale_stride from cuddle_int4_sizes, at least ceil(dim / group), the rest
  *            of a row 0; 16-byte aligned
  *   sqnorm : [n] f64, |row|^2 of what the row stands for; distances use it (NULL is allowed for DOT and lookups) */

@@ -28,9 +28,9 @@ def test_struct_layout():
     assert C.sizeof(_ffi.Int4RowsDesc) == 40
 
 
-@pytest.mark.parametrize("n,dim,group,want", [(1, 1, 32, (512, 4)), (16, 64, 64, (512, 2)), (17, 65, 64, (2048, 2)), (1000, 960, 64, (63 * 15 * 512, 16)),
-                                              (1000, 960, 32, (63 * 15 * 512, 32)), (10, 1536, 128, (24 * 512, 16)), (0, 8, 32, (0, 4)),
-                                              (3, 300, 128, (5 * 512, 4))])
+@pytest.mark.parametrize("n,dim,group,want", [(1, 1, 32, (512 + 16, 4)), (16, 64, 64, (512 + 16, 2)), (17, 65, 64, (2048, 2)), (1000, 960, 64, (63 * 15 * 512 + 16, 16)),
+                                              (1000, 960, 32, (63 * 15 * 512 + 16, 32)), (10, 1536, 128, (24 * 512, 16)), (0, 8, 32, (0, 4)),
+                                              (3, 300, 128, (5 * 512 + 16, 4))])
 def test_sizes(n, dim, group, want):
     assert _sizes(n, dim, group) == (_ffi.OK,) + want
 

@@ -2926,18 +2926,17 @@ struct DeviceGuard { // the calls below leave the caller's current device as it 
 
 unsigned grid_for(uint64_t blocks) { return (unsigned)std::min<uint64_t>(std::max<uint64_t>(blocks, 1), 1u << 20); }
 // Shape of the lookups: a row's pieces over at most 256 threads (grid.y parts of them), several rows per block where
-// they fit, four per thread where there are enough rows to fill the chip that way (four neighbouring 4-bit rows are the
-// same 128-byte lines: decoding 1M x 960 to f32 takes 829 us, 1196 with one row per block, 1036 with sixteen).
+// they fit, `each` per thread where there are enough rows to fill the chip that way.
 struct RowShape {
     uint32_t w, rpi, rpb;
     dim3 grid;
 };
-RowShape row_shape(uint32_t pieces, uint64_t rows) {
+RowShape row_shape(uint32_t pieces, uint64_t rows, uint32_t each = 4) {
     RowShape r;
     const uint32_t parts = (pieces + 255) / 256;
     r.w = (pieces + parts - 1) / parts;
     r.rpi = 256 / r.w;
-    r.rpb = rows * parts / r.rpi > 4096 ? r.rpi * 4 : r.rpi;
+    r.rpb = rows * parts / r.rpi > 4096 ? r.rpi * each : r.rpi;
     r.grid = dim3((unsigned)std::min<uint64_t>((rows + r.rpb - 1) / r.rpb, (1u << 20) / parts), parts); // far from 2^32 threads
     return r;
 }
@@ -3191,7 +3190,8 @@ extern "C" cuddle_status cuddle_int4_sizes(uint64_t n, uint32_t dim, uint32_t gr
     ST_TRY(check_dim(dim));
     ST_TRY(check_group(group));
     if (n >= 0xFFFFFFFFull) return fail(CUDDLE_ERR_UNSUPPORTED, "%llu rows: fewer than 2^32 - 1", (unsigned long long)n);
-    *code_bytes = (n + 15) / 16 * int4_units(dim) * kInt4UnitBytes;
+    const uint32_t units = int4_units(dim);
+    *code_bytes = (n + 15) / 16 * units * kInt4UnitBytes + (n && (units & 1) ? 16 : 0); // an odd last unit is read 16 bytes at a time
     *scale_stride = int4_gstride(dim, group);
     return CUDDLE_OK;
 }
@@ -3238,7 +3238,9 @@ extern "C" cuddle_status cuddle_int4_lookup_device(const cuddle_int4_rows *rows,
     DeviceGuard guard;
     ST_TRY(guard.enter(device_id));
     if (n_ids == 0) return CUDDLE_OK;
-    const RowShape sh = row_shape((rows->dim * type_size(out_type) + 15) / 16, n_ids);
+    // in order: two rows per thread, which share their 128-byte lines of codes (1M x 960 to f32: 920 us, 960 with four,
+    // 1196 with one)
+    const RowShape sh = row_shape((rows->dim * type_size(out_type) + 15) / 16, n_ids, d_ids ? 4 : 2);
     const bool vec = aligned16(d_out) && (uint64_t)rows->dim * type_size(out_type) % 16 == 0;
     with_type(out_type, [&](auto z) {
         using T = decltype(z);

@@ -8,12 +8,14 @@
 // A group whose scale rounds to zero has codes 0; a group that holds a NaN or an infinity gets s = NaN and codes 0,
 // so it decodes to NaN and every distance of the row is NaN.
 //
-// Layout. What a wave wants to load is what one matrix instruction eats: 16 rows x 64 components of int8, lane
-// (r = lane & 15, h = lane >> 4) holding 16 components of row r. So codes are stored in units of 16 rows x 64
-// components (512 bytes, rows of 32 bytes), units of a tile of 16 rows one after the other:
-//   byte h * 8 + i of a row's unit = component 8h + i in the low nibble, 32 + 8h + i in the high nibble (i < 8),
-// two's complement. A wave reads 8 bytes per lane, 512 contiguous bytes, and has both halves of the operand after a
-// shift and two masks; the code stays in the high nibble of its byte, so the products come out 16 times too large
+// Layout. What a wave wants to load is what matrix instructions eat: 16 rows x 64 components of int8 each, lane
+// (r = lane & 15, h = lane >> 4) holding 16 components of row r. So codes are stored by tiles of 16 rows and units of 64
+// components, 8 bytes of a unit per lane: byte i = component 8h + i in the low nibble, 32 + 8h + i in the high nibble
+// (i < 8), two's complement. Units come in pairs of 1024 bytes,
+//   byte r * 64 + h * 16 + (unit & 1) * 8 + i,
+// so that a wave reads 16 bytes per lane, 1 KB in a run, and a row has 64 bytes in a run (fetching a row by id: half the
+// lines that single units of 32 bytes a row would touch). An odd last unit has 512 bytes, byte r * 32 + h * 8 + i. The
+// operand is made with a shift and two masks; the code stays in the high nibble of its byte, so the products come out 16 times too large
 // (an exact factor, taken out at the end). Scales are row-major: [rows][gstride] bf16; gstride is the number of groups
 // rounded up to 2, 4 or 8, so that the scales of neighbouring units come in one aligned load.
 #pragma once
@@ -27,6 +29,12 @@ typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 constexpr uint32_t kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2;
 constexpr uint32_t kInt4Unit = 64;      // components per unit
 constexpr uint32_t kInt4UnitBytes = 512; // 16 rows x 32 bytes
+
+// Offset in a tile of byte b = 8h + i of row r's unit u.
+__device__ __forceinline__ uint32_t int4_code_at(uint32_t units, uint32_t u, uint32_t r, uint32_t b) {
+    if (u == units - 1 && !(u & 1)) return u * kInt4UnitBytes + r * 32 + b;
+    return (u >> 1) * (2 * kInt4UnitBytes) + r * 64 + (b >> 3) * 16 + (u & 1) * 8 + (b & 7);
+}
 
 __host__ __device__ __forceinline__ uint32_t int4_units(uint32_t dim) { return (dim + kInt4Unit - 1) / kInt4Unit; }
 __host__ __device__ __forceinline__ uint32_t int4_gstride(uint32_t dim, uint32_t group) {
@@ -159,7 +167,7 @@ int4_encode_kernel(const T *x, uint64_t stride, uint64_t first, uint64_t count, 
             const uint32_t q0 = (uint32_t)__shfl_xor((int)p0, 4, 64), q1 = (uint32_t)__shfl_xor((int)p1, 4, 64);
             if (act && u < units) {
                 if (jj < 4)
-                    *reinterpret_cast<uint2 *>(codes + (t * units + u) * kInt4UnitBytes + r * 32 + jj * 8) = make_uint2(p0 | q0 << 4, p1 | q1 << 4);
+                    *reinterpret_cast<uint2 *>(codes + t * units * kInt4UnitBytes + int4_code_at(units, u, r, jj * 8)) = make_uint2(p0 | q0 << 4, p1 | q1 << 4);
                 const uint32_t g = e0 / group;
                 if (e0 % group == 0 && g < gs) scales[row * gs + g] = sb;
             }
@@ -233,7 +241,8 @@ int4_lookup_kernel(const uint8_t *codes, const uint16_t *scales, uint64_t n, uin
     constexpr int N = 16 / sizeof(T), W = N / 4; // components, words of codes
     const uint32_t units = int4_units(dim), gs = int4_gstride(dim, group), rr = threadIdx.x / w, e0 = (blockIdx.y * w + threadIdx.x - rr * w) * N;
     if (rr >= rpi || e0 >= dim) return;
-    const uint32_t e6 = e0 & 63, code_at = (e0 >> 6) * kInt4UnitBytes + (e6 & 31), g = e0 / group, up = e6 < 32 ? 4 : 0;
+    const uint32_t e6 = e0 & 63, g = e0 / group, up = e6 < 32 ? 4 : 0;
+    const uint32_t code_at = int4_code_at(units, e0 >> 6, 0, e6 & 31), pitch = int4_code_at(units, e0 >> 6, 1, e6 & 31) - code_at; // bytes between rows
     for (uint64_t t0 = (uint64_t)blockIdx.x * rpb; t0 < n_ids; t0 += (uint64_t)gridDim.x * rpb) {
         const uint64_t te = min(t0 + rpb, n_ids);
         for (uint64_t t1 = t0 + rr; t1 < te; t1 += U * rpi) {
@@ -251,7 +260,7 @@ int4_lookup_kernel(const uint8_t *codes, const uint16_t *scales, uint64_t n, uin
                 for (int i = 0; i < W; ++i) c[u].v[i] = 0;
                 sb[u] = 0;
                 if (row[u] != kNoRow) {
-                    c[u] = *reinterpret_cast<const Pack<uint32_t, W> *>(codes + (row[u] >> 4) * units * kInt4UnitBytes + (uint32_t)(row[u] & 15) * 32 + code_at);
+                    c[u] = *reinterpret_cast<const Pack<uint32_t, W> *>(codes + (row[u] >> 4) * units * kInt4UnitBytes + (uint32_t)(row[u] & 15) * pitch + code_at);
                     sb[u] = scales[row[u] * gs + g];
                 }
             }
@@ -596,6 +605,7 @@ int4_distance_kernel(Int4DistArgs a) {
         uint2 w[T][P];
         Pack<uint16_t, SC> sc[T];
     };
+    const uint32_t pair_at = r * 64 + h * 16, single_at = r * 32 + h * 8;
     auto request = [&](uint64_t g, uint32_t ub, Piece &v) {
 #pragma unroll
         for (int t = 0; t < T; ++t) { // tile and pointers are the wave's, only the offsets are the lane's
@@ -604,13 +614,13 @@ int4_distance_kernel(Int4DistArgs a) {
             const uint8_t *sp = reinterpret_cast<const uint8_t *>(a.scales + tile * 16 * a.gs);
             const uint32_t so = min(r, (uint32_t)min(a.n - 1 - tile * 16, (uint64_t)15)) * a.gs * 2; // rows past the last: the last
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const uint8_t *at = wp + (uint64_t)min(ub + p, a.units - 1) * kInt4UnitBytes + (r * 32 + h * 8);
-                if (NT) {
-                    const uint64_t b = __builtin_nontemporal_load(reinterpret_cast<const uint64_t *>(at));
-                    v.w[t][p] = make_uint2((uint32_t)b, (uint32_t)(b >> 32));
-                } else
-                    v.w[t][p] = *reinterpret_cast<const uint2 *>(at);
+            for (int p = 0; p < P; p += 2) { // a pair of units; of an odd last one the second half is not its own and meets zero digits
+                const uint32_t u = min(ub + p, (a.units - 1) & ~1u);
+                const uint8_t *at = wp + (uint64_t)u * kInt4UnitBytes + (u == a.units - 1 ? single_at : pair_at);
+                typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));
+                const u32x4_8 b = NT ? __builtin_nontemporal_load(reinterpret_cast<const u32x4_8 *>(at)) : *reinterpret_cast<const u32x4_8 *>(at);
+                v.w[t][p] = make_uint2(b[0], b[1]);
+                v.w[t][p + 1] = make_uint2(b[2], b[3]);
             }
             v.sc[t] = *reinterpret_cast<const Pack<uint16_t, SC> *>(sp + 2 * (ub * 64 / G) + so); // gs is a multiple of SC: these are the row's own
         }

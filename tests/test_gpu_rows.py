@@ -326,7 +326,8 @@ def _check_grad(got, g, ids, n, scale, out, prev=None):
 
 
 @pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32), (F32, BF16), (F16, BF16)])
-@pytest.mark.parametrize("n,d,t", [(1, 1, 1), (1, 64, 300), (10, 33, 5), (50, 128, 2048), (300, 130, 2049), (70_000, 16, 5000), (3, 960, 700), (257, 8, 10_000), (40, 24, 3840), (40, 24, 3841),
+@pytest.mark.parametrize("n,d,t", [(1, 1, 1), (1, 64, 300), (10, 33, 5), (50, 128, 2048), (300, 130, 2049), (70_000, 16, 5000), (3, 960, 700), (257, 8, 10_000), (40, 24, 3840), (40, 24, 8192), (40, 24, 8193), (40, 24, 16_384), (40, 24, 16_385), (100_000, 8, 16_383),
+                                   (900_000, 8, 66_000), (3_000_000, 4, 30_000), (1_000, 8, 70_000),
                                    (1_200_000, 4, 140_000), (2, 520, 200_000)])
 def test_rows_grad(gpu, n, d, t, dtype, out):
     rng = np.random.default_rng(n + d + t)

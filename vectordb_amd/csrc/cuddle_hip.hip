@@ -3410,7 +3410,7 @@ namespace {
 // Work space of a gradient: sorted (row, place) pairs (two buffers for more than one pass), tile histograms, the map of
 // named rows, the parts of runs that chunks cut.
 struct GradWs {
-    uint32_t R = 0, chunks = 0, tile = 0;
+    uint32_t R = 0, chunks = 0, tile = 0, tiles = 0, passes = 0, bits = 0;
     size_t place[2] = {0, 0}, hist = 0, total = 0, named = 0, part = 0, bytes = 0;
 };
 GradWs grad_ws(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
@@ -3429,7 +3429,12 @@ GradWs grad_ws(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
     for (int i = 0; i < (small ? 1 : 2); ++i) w.place[i] = take(n_ids * 8);
     if (!small) {
         w.tile = n_ids <= (256u << 10) ? 1024 : 4096;
-        w.hist = take(((n_ids + w.tile - 1) / w.tile << kSortMaxBits) * 4);
+        uint32_t row_bits = 1;
+        while (n_rows >> row_bits) ++row_bits; // keys are 0 .. n_rows
+        w.passes = (row_bits + kSortMaxBits - 1) / kSortMaxBits;
+        w.bits = (row_bits + w.passes - 1) / w.passes;
+        w.tiles = (uint32_t)((n_ids + w.tile - 1) / w.tile);
+        w.hist = take(((uint64_t)w.tiles << w.bits) * 4);
         w.total = take(4u << kSortMaxBits);
         w.named = take(n_rows);
     }
@@ -3479,32 +3484,36 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
     }
     uint8_t *ws = (uint8_t *)d_ws;
     const uint32_t t = (uint32_t)n_ids;
-    uint32_t row_bits = 1;
-    while (n_rows >> row_bits) ++row_bits; // keys are 0 .. n_rows
     int cur = 0;
     uint8_t *named = nullptr;
     if (t <= kSortSmall) {
+        uint32_t row_bits = 1;
+        while (n_rows >> row_bits) ++row_bits; // keys are 0 .. n_rows
         const unsigned zero_blocks = add ? 0 : (unsigned)std::min<uint64_t>((grad_bytes + 65535) / 65536, 4096);
         with_id(id_bits, [&](auto zi) {
             using I = decltype(zi);
-            hipLaunchKernelGGL(rows_sort_small_kernel<I>, dim3(1 + zero_blocks), dim3(1024), 0, s, (const I *)d_ids, t, n_rows, (row_bits + 7) / 8,
+            static std::once_flag once[kMaxDevices];
+            std::call_once(once[device_id & (kMaxDevices - 1)], [] {
+                (void)hipFuncSetAttribute((const void *)rows_sort_small_kernel<I>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sort_small_lds(kSortSmall));
+            });
+            hipLaunchKernelGGL(rows_sort_small_kernel<I>, dim3(1 + zero_blocks), dim3(1024), sort_small_lds(t), s, (const I *)d_ids, t, n_rows, (row_bits + 7) / 8,
                                (uint2 *)(ws + w.place[0]), d_grad, grad_bytes);
         });
     } else {
         uint32_t *hist = (uint32_t *)(ws + w.hist), *total = (uint32_t *)(ws + w.total);
-        const uint32_t tiles = (t + w.tile - 1) / w.tile, passes = (row_bits + kSortMaxBits - 1) / kSortMaxBits, bits = (row_bits + passes - 1) / passes;
-        const unsigned clear = add ? 0 : (unsigned)std::min<uint64_t>((n_rows + 16383) / 16384, 256);
         named = add ? nullptr : ws + w.named;
+        const unsigned clear = add ? 0 : (unsigned)std::min<uint64_t>((n_rows + 16383) / 16384, 256);
+        const bool scan = w.tiles > kSortSumTiles;
         auto sort = [&](auto items) {
             constexpr int J = decltype(items)::value;
-            for (uint32_t p = 0; p < passes; ++p, cur ^= 1) {
-                const uint32_t shift = p * bits;
+            for (uint32_t p = 0; p < w.passes; ++p, cur ^= 1) {
                 uint2 *out = (uint2 *)(ws + w.place[cur ^ 1]);
-                const void *in = ws + w.place[cur];
+                const uint32_t shift = p * w.bits;
                 auto pass = [&](auto hist_kernel, auto scatter_kernel, const void *src, unsigned extra, uint8_t *map) {
-                    hipLaunchKernelGGL(hist_kernel, dim3(tiles + extra), dim3(256), 0, s, src, t, n_rows, shift, bits, tiles, hist, ws + w.named);
-                    hipLaunchKernelGGL(rows_sort_scan_kernel, dim3(((1u << bits) + 63) / 64), dim3(1024), 0, s, hist, tiles, 1u << bits, total);
-                    hipLaunchKernelGGL(scatter_kernel, dim3(tiles), dim3(256), 0, s, src, t, n_rows, shift, bits, hist, total, out, map);
+                    hipLaunchKernelGGL(hist_kernel, dim3(w.tiles + extra), dim3(256), 0, s, src, t, n_rows, shift, w.bits, w.tiles, hist, map);
+                    if (scan) hipLaunchKernelGGL(rows_sort_scan_kernel, dim3(((1u << w.bits) + 63) / 64), dim3(1024), 0, s, hist, w.tiles, 1u << w.bits, total);
+                    hipLaunchKernelGGL(scatter_kernel, dim3(w.tiles), dim3(256), 0, s, src, t, n_rows, shift, w.bits, w.tiles, (const uint32_t *)hist,
+                                       (const uint32_t *)(scan ? total : nullptr), out, map);
                 };
                 if (p == 0)
                     with_id(id_bits, [&](auto zi) {
@@ -3512,7 +3521,7 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
                         pass(rows_sort_hist_kernel<J, true, I>, rows_sort_scatter_kernel<J, true, I>, d_ids, clear, named);
                     });
                 else
-                    pass(rows_sort_hist_kernel<J, false, int32_t>, rows_sort_scatter_kernel<J, false, int32_t>, in, 0u, (uint8_t *)nullptr);
+                    pass(rows_sort_hist_kernel<J, false, int32_t>, rows_sort_scatter_kernel<J, false, int32_t>, ws + w.place[cur], 0u, (uint8_t *)nullptr);
             }
         };
         if (w.tile == 1024) sort(std::integral_constant<int, 4>{});

@@ -1022,9 +1022,11 @@ __device__ __forceinline__ uint32_t wave_rank(uint32_t d, bool in, uint32_t bits
     return at;
 }
 
-// Few places: block 0 sorts them all in LDS, 8 bits per pass, 16 waves with at most 256 keys each; the
-// other blocks zero the gradient meanwhile (zero == nullptr: it is added to). block 1024.
-constexpr uint32_t kSortSmall = 3840; // what 64 KB of LDS hold beside the counters
+// Few places: block 0 sorts them all in LDS, 8 bits per pass, 16 waves with an equal share each; the other blocks zero
+// the gradient meanwhile (zero == nullptr: it is added to). The keys stay where they are, 2-byte places move. block 1024,
+// dynamic LDS sort_small_lds(t).
+constexpr uint32_t kSortSmall = 8192; // beyond, the launches of the passes cost less (8000 places among 50 000 rows 28 us, 16 000 44 against 34)
+__host__ __device__ __forceinline__ uint32_t sort_small_lds(uint32_t t) { return (t + 1) / 2 * 16 + (16 * 256 + 257) * 4; }
 template <class I>
 __global__ void __launch_bounds__(1024)
 rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passes, uint2 *out, void *zero, uint64_t zero_bytes) {
@@ -1032,26 +1034,28 @@ rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passe
         zero_share(zero, zero_bytes, blockIdx.x - 1, gridDim.x - 1);
         return;
     }
-    __shared__ uint32_t key[2][kSortSmall];
-    __shared__ uint16_t pos[2][kSortSmall];
-    __shared__ uint32_t off[16][256];
-    __shared__ uint32_t tot[257];
+    extern __shared__ uint32_t smem_sort[];
+    uint32_t *off = smem_sort, *tot = off + 16 * 256, *key = tot + 257;
+    uint16_t *pos[2] = {reinterpret_cast<uint16_t *>(key + (t + 1) / 2 * 2), nullptr};
+    pos[1] = pos[0] + (t + 1) / 2 * 2;
     const uint32_t tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-    const uint32_t per = (((t + 15) / 16) + 63) & ~63u, b = w * per; // keys of a wave
+    const uint32_t per = (((t + 15) / 16) + 63) & ~63u, b = w * per; // places of a wave
+    uint32_t *mine = off + w * 256;
     for (uint32_t i = tid; i < t; i += 1024) {
-        key[0][i] = grad_key(ids, i, n_rows);
+        key[i] = grad_key(ids, i, n_rows);
         pos[0][i] = (uint16_t)i;
     }
-    uint32_t cur = 0;
-    for (uint32_t p = 0; p < passes; ++p, cur ^= 1) {
+    for (uint32_t p = 0; p < passes; ++p) {
         const uint32_t shift = 8 * p;
-        for (uint32_t i = tid; i < 16 * 256; i += 1024) (&off[0][0])[i] = 0;
+        const uint16_t *from = pos[p & 1];
+        uint16_t *to = pos[(p & 1) ^ 1];
+        for (uint32_t i = tid; i < 16 * 256; i += 1024) off[i] = 0;
         __syncthreads();
-        for (uint32_t i = b + lane; i < min(b + per, t); i += 64) atomicAdd(&off[w][(key[cur][i] >> shift) & 255], 1u);
+        for (uint32_t i = b + lane; i < min(b + per, t); i += 64) atomicAdd(&mine[(key[from[i]] >> shift) & 255], 1u);
         __syncthreads();
         if (tid < 256) {
             uint32_t run = 0;
-            for (int v = 0; v < 16; ++v) run += off[v][tid];
+            for (int v = 0; v < 16; ++v) run += off[v * 256 + tid];
             tot[tid] = run;
         }
         __syncthreads();
@@ -1060,33 +1064,31 @@ rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passe
         if (tid < 256) {
             uint32_t run = tot[tid];
             for (int v = 0; v < 16; ++v) {
-                const uint32_t c = off[v][tid];
-                off[v][tid] = run;
+                const uint32_t c = off[v * 256 + tid];
+                off[v * 256 + tid] = run;
                 run += c;
             }
         }
         __syncthreads();
-        for (uint32_t i0 = b; i0 < b + per; i0 += 64) {
+        for (uint32_t i0 = b; i0 < min(b + per, t); i0 += 64) {
             const uint32_t i = i0 + lane;
             const bool in = i < t;
-            const uint32_t k = in ? key[cur][i] : 0u;
-            const uint32_t at = wave_rank((k >> shift) & 255, in, 8, off[w]);
-            if (in) {
-                key[cur ^ 1][at] = k;
-                pos[cur ^ 1][at] = pos[cur][i];
-            }
+            const uint16_t f = in ? from[i] : (uint16_t)0;
+            const uint32_t at = wave_rank(((in ? key[f] : 0u) >> shift) & 255, in, 8, mine);
+            if (in) to[at] = f;
         }
         __syncthreads();
     }
-    for (uint32_t i = tid; i < t; i += 1024) out[i] = make_uint2(key[cur][i], pos[cur][i]);
+    const uint16_t *sorted = pos[passes & 1];
+    for (uint32_t i = tid; i < t; i += 1024) out[i] = make_uint2(key[sorted[i]], sorted[i]);
 }
 
-// More places: per pass (up to 10 bits) a histogram per tile of J * 256 places, the histograms' prefix sums, the scatter.
-// J = 4 up to a million places (the tiles' waves rank their places one 64 after the other: 64K places 15 us with J = 16,
-// 6 us with 4), 16 beyond (the histograms grow with the tiles).
-// The first pass reads the ids themselves. The first histogram launch also clears the map of rows that ids name
-// (one byte each), the first scatter fills it in; the gradient kernel zeroes the rows it does not hold.
-constexpr uint32_t kSortMaxBits = 10;
+// More places: passes of up to 10 bits over tiles of J * 256 places, a count of the digits per tile (the first also clears
+// the map of rows that ids name, one byte each), then the scatter. Up to kSortSumTiles tiles a scatter's block adds the
+// counts up itself, beyond that a scan between the two does it. (Counting the next pass's digits in the scatter, by atomic
+// adds where the places land, measured slower: 64K skewed places 17 us for scatter and count, against 7 + 4.) J = 4 up to 256 K places (the tiles' waves rank their places one 64 after the other: 64K places 15 us with J = 16, 7
+// with 4), 16 beyond (the counts grow with the tiles).
+constexpr uint32_t kSortMaxBits = 10, kSortSumTiles = 64;
 
 template <int J, bool FIRST, class I>
 __global__ void __launch_bounds__(256)
@@ -1142,16 +1144,31 @@ rows_sort_scan_kernel(uint32_t *hist, uint32_t tiles, uint32_t bins, uint32_t *t
     }
 }
 
+// total == nullptr: hist holds plain counts, to be added up here.
 template <int J, bool FIRST, class I>
 __global__ void __launch_bounds__(256)
-rows_sort_scatter_kernel(const void *src, uint32_t t, uint64_t n_rows, uint32_t shift, uint32_t bits, const uint32_t *hist,
-                         const uint32_t *total, uint2 *out, uint8_t *named) {
+rows_sort_scatter_kernel(const void *src, uint32_t t, uint64_t n_rows, uint32_t shift, uint32_t bits, uint32_t tiles, const uint32_t *hist, const uint32_t *total,
+                         uint2 *out, uint8_t *named) {
     __shared__ uint32_t off[4][1u << kSortMaxBits];
     __shared__ uint32_t tot[(1u << kSortMaxBits) + 1];
+    __shared__ uint32_t before[1u << kSortMaxBits]; // places of the digit in the tiles before
     const uint32_t tid = threadIdx.x, w = tid >> 6, lane = tid & 63, bins = 1u << bits;
     for (uint32_t i = tid; i < bins; i += 256) {
         off[0][i] = off[1][i] = off[2][i] = off[3][i] = 0;
-        tot[i] = total[i];
+        if (total) {
+            tot[i] = total[i];
+            before[i] = hist[(uint64_t)blockIdx.x * bins + i];
+        } else {
+            uint32_t all = 0, bef = 0;
+#pragma unroll 16
+            for (uint32_t u = 0; u < tiles; ++u) {
+                const uint32_t v = hist[(uint64_t)u * bins + i];
+                all += v;
+                bef += u < blockIdx.x ? v : 0u;
+            }
+            tot[i] = all;
+            before[i] = bef;
+        }
     }
     __syncthreads();
     const uint32_t b = blockIdx.x * (J * 256) + w * (J * 64);
@@ -1175,7 +1192,7 @@ rows_sort_scatter_kernel(const void *src, uint32_t t, uint64_t n_rows, uint32_t 
     wave0_exclusive_scan_lds(tot, bins);
     __syncthreads();
     for (uint32_t i = tid; i < bins; i += 256) {
-        uint32_t run = tot[i] + hist[(uint64_t)blockIdx.x * bins + i];
+        uint32_t run = tot[i] + before[i];
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             const uint32_t c = off[v][i];

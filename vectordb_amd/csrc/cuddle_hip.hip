@@ -2983,7 +2983,7 @@ template <class F> void with_id(uint32_t bits, F f) {
 constexpr size_t kAlign = 256;
 size_t round_ws(size_t b) { return (b + kAlign - 1) & ~(kAlign - 1); }
 
-constexpr uint32_t int4_lds_kb(int qt) { return qt >= 3 ? 144u : 64u; } // digits per block: one block of 8 waves per CU, or two of 4 and more
+constexpr uint32_t int4_lds_kb(int qt) { return qt >= 8 ? 128u : qt >= 3 ? 144u : 64u; } // digits per block: one large block per CU, or several
 // Up to four queries whose digits fit a block's LDS: the distance kernel makes them itself. A round of a call is fused if
 // its queries are this few, so a call of more queries lays out room for digits also for a last, smaller round.
 bool int4_fused(uint64_t nq, uint32_t dim) { return nq <= 4 && (int4_units(dim) + 7) / 8 * 8 <= int4_lds_kb(1); }
@@ -3113,9 +3113,9 @@ void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStre
         return;
     }
     uint32_t best = 1, cost = ~0u;
-    for (uint32_t qt : {1u, 2u, 3u, 4u, 6u, 8u}) {
-        if (qt > 4 && a.units < 6) break; // short rows: the finish weighs as much as the products, and four waves per SIMD
-                                          // (QT <= 4) hide more of it than two (1M x 128, 100 queries: 167 us against 206)
+    for (uint32_t qt : {1u, 2u, 3u, 4u, 5u, 8u}) {
+        if (qt > 5 && a.units < 6) break; // short rows: the finish weighs as much as the products (1M x 128, 100 queries: 167 us
+                                          // with 4 and 149 with 5, against 206 with 8)
         const uint32_t ys = (quads + qt - 1) / qt;
         const bool whole = a.units <= int4_lds_kb((int)qt) / qt; // else the digits are fetched anew for every 256 rows: about as much again
         const uint32_t c = ys * (qt * (whole ? 1 : 2) + 1);
@@ -3129,10 +3129,9 @@ void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStre
     case 2: int4_launch<G, 2, 2, 2, false, false, float>(a, s); break;
     case 3: int4_launch<G, 3, 2, 2, false, false, float>(a, s); break;
     case 4: int4_launch<G, 4, 2, 2, false, false, float>(a, s); break;
-    case 6: int4_launch<G, 6, 2, 2, false, false, float>(a, s); break;
+    case 5: int4_launch<G, 5, 2, 2, false, false, float>(a, s); break;
     default:
-        if (a.units >= 4) int4_launch<G, 8, 2, 4, false, false, float>(a, s);
-        else int4_launch<G, 8, 2, 2, false, false, float>(a, s);
+        int4_launch<G, 8, 1, 4, false, false, float>(a, s);
         break;
     }
 }

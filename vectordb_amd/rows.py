@@ -56,15 +56,16 @@ def _id_bits(ids: torch.Tensor) -> int:
 
 
 _NO_CTX = contextlib.nullcontext()
+# the current stream's handle without a Stream object around it, where torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _enter(dev: torch.device, stream, *inputs: torch.Tensor):
     """(context, device index, hipStream_t) for work on `dev` and `stream`: inside the context torch's copies and
     allocations belong to the stream. Inputs used on a stream that is not the current one are kept for it."""
     index = dev.index if dev.index is not None else torch.cuda.current_device()
-    cur = torch.cuda.current_stream(index)
-    if stream is None or stream == cur:
-        return _NO_CTX, index, cur.cuda_stream
+    if stream is None or stream.cuda_stream == _raw_stream(index):
+        return _NO_CTX, index, _raw_stream(index)
     for t in inputs:
         t.record_stream(stream)
     return torch.cuda.stream(stream), index, stream.cuda_stream

@@ -2983,7 +2983,7 @@ template <class F> void with_id(uint32_t bits, F f) {
 constexpr size_t kAlign = 256;
 size_t round_ws(size_t b) { return (b + kAlign - 1) & ~(kAlign - 1); }
 
-constexpr uint32_t int4_lds_kb(int qt) { return qt >= 8 ? 128u : qt >= 3 ? 144u : 64u; } // digits per block: one large block per CU, or several
+constexpr uint32_t int4_lds_kb(int qt) { return qt >= 5 ? 128u : qt >= 3 ? 144u : 64u; } // digits per block: one large block per CU, or several
 // Up to four queries whose digits fit a block's LDS: the distance kernel makes them itself. A round of a call is fused if
 // its queries are this few, so a call of more queries lays out room for digits also for a last, smaller round.
 bool int4_fused(uint64_t nq, uint32_t dim) { return nq <= 4 && (int4_units(dim) + 7) / 8 * 8 <= int4_lds_kb(1); }
@@ -3053,11 +3053,16 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
 }
 
 // Launch shapes of the distance kernel. One quartet of queries: codes are the bound, so many of them are requested at a
-// time (16 pieces of 512 bytes per wave). More: QT quartets per wave, the count among those built that costs least,
-// pairs of (row, query) at about 27 cycles and the unpacking of the codes, once per QT, at about as much.
+// time (four pieces of 1 KB per wave). More: QT quartets per wave, the count among those built that costs least.
+// A wave's pass over its codes unpacks them once and multiplies them QT times; unpacking, addresses and the wait cost
+// about as much as three quartets' products (1M x 960, one pass: 140 us with 5 quartets, 190 with 8, 114 with 4, 98 with
+// 3). 20 queries: 161 us with 5, 210 with 8; 64: 401 with 8, 498 with 5, 471 with 4; 100: 682 with 5, 730 with 8, 779
+// with 4. Six and seven quartets were built and won nowhere by more than 4 %. Digits that do not fit the block's LDS at
+// once are fetched anew for every 256 rows, from the L2, and change nothing in the order (100k x 4096, 64 queries: 221 us
+// with 8, 264 with 5, 289 with 4).
 template <int G, int QT, int T, int P, bool FUSED, bool NT, class TQ>
 void int4_launch(Int4DistArgs a, hipStream_t s) {
-    constexpr uint32_t NW = int4_block(QT) / 64;
+    constexpr uint32_t NW = int4_block(QT, T) / 64;
     a.ku = std::min<uint32_t>((a.units + P - 1) / P * P, int4_lds_kb(QT) / QT / P * P);
     a.ys = ((a.nq + 3) / 4 + QT - 1) / QT;
     const uint64_t groups = (a.stiles + NW * T - 1) / (NW * T);
@@ -3077,7 +3082,7 @@ void int4_launch(Int4DistArgs a, hipStream_t s) {
     uint64_t k = known.load(std::memory_order_relaxed);
     if (k >> 32 != lds) {
         int n = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, int4_block(QT), lds) != hipSuccess || n < 1) {
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, int4_block(QT, T), lds) != hipSuccess || n < 1) {
             (void)hipGetLastError();
             n = 1;
         }
@@ -3089,13 +3094,9 @@ void int4_launch(Int4DistArgs a, hipStream_t s) {
     xs = std::min<uint64_t>(groups, xs);
     if (a.ys > 1) xs = (xs + 7) / 8 * 8;
     a.xs = (uint32_t)xs;
-    hipLaunchKernelGGL((int4_distance_kernel<G, QT, T, P, FUSED, NT, TQ>), dim3((unsigned)(a.xs * a.ys)), dim3(int4_block(QT)), lds, s, a);
+    hipLaunchKernelGGL((int4_distance_kernel<G, QT, T, P, FUSED, NT, TQ>), dim3((unsigned)(a.xs * a.ys)), dim3(int4_block(QT, T)), lds, s, a);
 }
 
-#ifndef QT_T
-#define QT_T 2
-#define QT_P 4
-#endif
 template <int G>
 void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStream_t s) {
     const uint32_t quads = (a.nq + 3) / 4;
@@ -3107,18 +3108,14 @@ void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStre
             const bool nt = (a.n + 15) / 16 * a.units * kInt4UnitBytes > (256ull << 20) && !a.stride;
             if (few_units && nt) int4_launch<G, 1, 4, 2, true, true, TQ>(a, s);
             else if (few_units) int4_launch<G, 1, 4, 2, true, false, TQ>(a, s);
-            else if (nt) int4_launch<G, 1, QT_T, QT_P, true, true, TQ>(a, s);
-            else int4_launch<G, 1, QT_T, QT_P, true, false, TQ>(a, s);
+            else if (nt) int4_launch<G, 1, 2, 4, true, true, TQ>(a, s);
+            else int4_launch<G, 1, 2, 4, true, false, TQ>(a, s);
         });
         return;
     }
-    uint32_t best = 1, cost = ~0u;
+    uint32_t best = 1, cost = ~0u; // (of equal costs the larger: its codes are unpacked less often)
     for (uint32_t qt : {1u, 2u, 3u, 4u, 5u, 8u}) {
-        if (qt > 5 && a.units < 6) break; // short rows: the finish weighs as much as the products (1M x 128, 100 queries: 167 us
-                                          // with 4 and 149 with 5, against 206 with 8)
-        const uint32_t ys = (quads + qt - 1) / qt;
-        const bool whole = a.units <= int4_lds_kb((int)qt) / qt; // else the digits are fetched anew for every 256 rows: about as much again
-        const uint32_t c = ys * (qt * (whole ? 1 : 2) + 1);
+        const uint32_t c = (quads + qt - 1) / qt * (qt + 3);
         if (c <= cost) {
             cost = c;
             best = qt;
@@ -3129,7 +3126,12 @@ void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStre
     case 2: int4_launch<G, 2, 2, 2, false, false, float>(a, s); break;
     case 3: int4_launch<G, 3, 2, 2, false, false, float>(a, s); break;
     case 4: int4_launch<G, 4, 2, 2, false, false, float>(a, s); break;
-    case 5: int4_launch<G, 5, 2, 2, false, false, float>(a, s); break;
+    case 5:
+        // rows of one or two units: a pair of units is all there is to request ahead, and two tiles keep the wave busy
+        // (1M x 128, 100 queries: 245 us against 295; from 192 dimensions on equal or slower, 100k x 4096: 455 against 345)
+        if (a.units < 3) int4_launch<G, 5, 2, 2, false, false, float>(a, s);
+        else int4_launch<G, 5, 1, 4, false, false, float>(a, s);
+        break;
     default:
         int4_launch<G, 8, 1, 4, false, false, float>(a, s);
         break;

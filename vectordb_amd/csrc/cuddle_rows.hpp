@@ -441,9 +441,9 @@ __device__ __forceinline__ double int4_add(double acc, i32x4_t c, double s) {
     return __builtin_fma(s, __builtin_fma((double)(c[2] + (c[3] << 8)), 65536.0, (double)(c[0] + (c[1] << 8))), acc);
 }
 
-// Threads. Eight quartets: sixteen waves around one copy of the digits (1M x 960, 64 queries: 472 us, 496 with eight waves
-// of two tiles each).
-__host__ __device__ constexpr int int4_block(int qt) { return qt >= 8 ? 1024 : qt >= 3 ? 512 : 256; }
+// Threads. Five and eight quartets of one tile: sixteen waves around one copy of the digits (1M x 960, 64 queries: 472 us,
+// 496 with eight waves of two tiles each; 20 queries: 196 and 215).
+__host__ __device__ constexpr int int4_block(int qt, int t) { return qt >= 5 && t == 1 ? 1024 : qt >= 3 ? 512 : 256; }
 
 struct Int4DistArgs {
     const uint8_t *codes;
@@ -524,15 +524,15 @@ __device__ __forceinline__ uint64_t int4_sampled(uint64_t i, uint32_t stride) {
 // one launch), else `ku` units at a time. Codes and scales of P units and T tiles are requested together; units past
 // the end repeat the last one against zero digits.
 // Few queries: bound by the codes' read. Many: by the six vector instructions that a group's products cost per pair
-// (two integer, two conversions, an f32 and an f64 fma; about 27 cycles against 16 of the matrix instruction).
+// (two integer, two conversions, two f64 fma): about 21 cycles, and 16 of the matrix instruction, that overlap little.
 // NT: codes that no cache holds until the next call are read without a claim to one (4 GiB: 6.3 -> 7.2 TB/s).
 // Blocks of the same rows and different queries are neighbours on one XCD, so that the rows' codes come from its L2.
 template <int G, int QT, int T, int P, bool FUSED, bool NT, class TQ>
-__global__ void __launch_bounds__(int4_block(QT), QT >= 3 ? 4 : 2) // at most 256 registers: products land in vector registers, not accumulators
+__global__ void __launch_bounds__(int4_block(QT, T), QT >= 3 ? 4 : 2) // at most 256 registers: products land in vector registers, not accumulators
 int4_distance_kernel(Int4DistArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t s_dig[];
     Int4Query *s_info = reinterpret_cast<Int4Query *>(s_dig + (size_t)a.ku * QT * 1024);
-    constexpr uint32_t NW = int4_block(QT) / 64;
+    constexpr uint32_t NW = int4_block(QT, T) / 64;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
     uint32_t x = blockIdx.x, y = 0;

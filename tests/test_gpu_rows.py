@@ -208,6 +208,29 @@ def test_search_by_sample(gpu, n, nq, k, metric):
     _check_search(R.int4_encode_device(x, 32), torch.randn((nq, 16), generator=gen, device="cuda"), k, metric)
 
 
+@pytest.mark.parametrize("k", [10, 1024])
+def test_search_in_rounds(gpu, k):
+    """More distances than a search holds at a time: the answers of all queries are those of a part of them at a time."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(k)
+    n, nq = 3_000_000, 402
+    r = R.int4_encode_device(torch.randn((n, 16), generator=gen, device="cuda"), 32)
+    q = torch.randn((nq, 16), generator=gen, device="cuda")
+    ids, dist, count = r.search_batch_device(q, k, "l2")
+    for at in range(0, nq, 67):
+        part = r.search_batch_device(q[at:at + 67], k, "l2")
+        assert all(torch.equal(w[at:at + 67], p) for w, p in zip((ids, dist, count), part))
+    _check_search(r, q[-6:], k, "l2")
+
+
+@pytest.mark.parametrize("n,nq,k", [(10_000_000, 10, 8), (4_000_000, 9, 1), (9_000_000, 6, 7), (2_000_000, 40, 100)])
+def test_search_by_small_sample(gpu, n, nq, k):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(nq)
+    x = torch.randn((n, 16), generator=gen, device="cuda")
+    _check_search(R.int4_encode_device(x, 32), torch.randn((nq, 16), generator=gen, device="cuda"), k, "l2")
+
+
 def test_search_by_sample_overflow_ties_nan(gpu):
     gen = torch.Generator(device="cuda")
     gen.manual_seed(3)

@@ -2996,7 +2996,7 @@ struct Int4Ws {
     uint64_t stiles = 0;
     size_t dig = 0, info = 0, dist = 0, sel[2] = {0, 0}, tau = 0, cnt = 0, list = 0, bytes = 0;
 };
-constexpr uint64_t kInt4DistBudget = 512ull << 20; // bytes of distances a search holds at a time (one quartet of queries at least)
+constexpr uint64_t kInt4DistBudget = 4ull << 30; // bytes of distances a search holds at a time, one quartet of queries at least (10M x 128, 100 queries: 2240 us with 512 MiB, 1240 with this)
 constexpr uint64_t kInt4MaxRound = 32768;          // queries per round (the launches' second grid dimension)
 // Sampling pays from about this many distances on (they are 128 MB to write and read again; the collection's extra
 // launches cost about 30 us).
@@ -3036,15 +3036,20 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
             w.sel[0] = take((size_t)qc * first * 8);
             w.sel[1] = take((size_t)qc * ((parts * k + kTopChunk - 1) / kTopChunk) * k * 8);
         }
-        // k of a sample of S rows bound k n / S of all: enough to expect 512 candidates, at most a sixteenth of the
-        // rows, but no fewer than expect half of the collection's room to be filled
+        // k of a sample of S rows bound about k n / S of all. A block finds the bound of a query in S / 1200 us and the
+        // collection takes 0.2 us per 1000 candidates: their sum is least at `expect` candidates per query (100 queries,
+        // k = 10: 1M x 128 with 512 178 us and with 2048 195; 10M x 128 3046 and 2228). The bound scatters (by a gamma
+        // distribution of shape k), and the collection's room is not to run out by chance: odds under 1e-6 per query.
+        // At most a sixteenth of the rows, but no fewer than expect half of that room to be filled.
         const uint64_t kn = (uint64_t)k * n;
-        const uint64_t rows = std::max<uint64_t>({4096, std::min<uint64_t>(kn / 512, n / 16), kn / (kTopChunk / 2)}), want = (rows + 15) / 16;
+        const double least = std::sqrt((double)kn * (double)((qc + 255) / 256) / (0.24 * (double)qc));
+        const uint64_t expect = (uint64_t)std::min(std::max(least, 512.0), k == 1 ? 512.0 : k < 8 ? 1024.0 : 2048.0);
+        const uint64_t rows = std::max<uint64_t>({4096, std::min<uint64_t>(kn / expect, n / 16), kn / (kTopChunk / 2)}), want = (rows + 15) / 16;
         if (qc * n >= kInt4SampleFrom && tiles / want >= 8) {
             w.stride = (uint32_t)(tiles / want);
             w.stiles = tiles / w.stride;
             w.tau = take(qc * 4);
-            w.cnt = take(qc * 4);
+            w.cnt = take(qc * kCountPitch * 4);
             w.list = take((size_t)qc * kTopChunk * 8);
         }
     }

@@ -445,6 +445,7 @@ __device__ __forceinline__ double int4_add(double acc, i32x4_t c, double s) {
 // 496 with eight waves of two tiles each; 20 queries: 196 and 215).
 __host__ __device__ constexpr int int4_block(int qt, int t) { return qt >= 5 && t == 1 ? 1024 : qt >= 3 ? 512 : 256; }
 
+constexpr uint32_t kCountPitch = 32; // counters of candidates stand 128 bytes apart: atomics on one line wait for each other
 struct Int4DistArgs {
     const uint8_t *codes;
     const uint16_t *scales;
@@ -462,7 +463,7 @@ struct Int4DistArgs {
     // search: either a sample of the tiles (dist[q][16 i + r] = row r of the i-th sampled tile, NaN past the last row) ...
     uint64_t stiles;         // tiles to visit: all, or the sample
     uint32_t stride;         // 0, or a sampled tile out of every `stride`
-    // ... or the candidates: rows whose key does not exceed tau[q] go to list[q][cap] in any order, cnt[q] counts them
+    // ... or the candidates: rows whose key does not exceed tau[q] go to list[q][cap] in any order, cnt[q * kCountPitch] counts them
     const uint32_t *tau;
     uint32_t *cnt;
     uint64_t *list;
@@ -546,7 +547,7 @@ int4_distance_kernel(Int4DistArgs a) {
     Int4Test *s_test = reinterpret_cast<Int4Test *>(s_tau + QT * 4);
     if (a.redo) { // uniform over the block
         bool any = false;
-        for (uint32_t q = y * QT * 4; q < min((y + 1) * QT * 4, a.nq); ++q) any |= a.redo[q] > a.cap;
+        for (uint32_t q = y * QT * 4; q < min((y + 1) * QT * 4, a.nq); ++q) any |= a.redo[q * kCountPitch] > a.cap;
         if (!any) return;
     }
     if (a.tau && tid < QT * 4) s_tau[tid] = a.tau[min(y * QT * 4 + tid, a.nq - 1)];
@@ -562,7 +563,7 @@ int4_distance_kernel(Int4DistArgs a) {
     auto flush = [&](uint32_t count) { // the first `count` <= 64
         if (lane < count) {
             const Int4Held c = s_held[lane];
-            const uint32_t at = atomicAdd(&a.cnt[c.q], 1u);
+            const uint32_t at = atomicAdd(&a.cnt[c.q * kCountPitch], 1u);
             if (at < a.cap) a.list[(uint64_t)c.q * a.cap + at] = (uint64_t)c.key << 32 | c.row;
         }
     };
@@ -868,7 +869,7 @@ int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint3
                        uint32_t cap) {
     __shared__ uint32_t keys[kTopChunk];
     __shared__ TopkLds s;
-    if (redo && redo[blockIdx.y] <= cap) return;
+    if (redo && redo[blockIdx.y * kCountPitch] <= cap) return;
     const uint32_t tid = threadIdx.x;
     for (uint32_t part = blockIdx.x; part < parts; part += gridDim.x) {
         const uint64_t base = (uint64_t)part * chunk;
@@ -905,7 +906,7 @@ int4_topk_bound_kernel(const float *dist, uint64_t dstride, uint32_t items, uint
         block_kth_key(items, k, [&](uint32_t i) { return f32_key(df[i]); }, s, T, budget);
     if (threadIdx.x == 0) {
         tau[blockIdx.x] = T;
-        cnt[blockIdx.x] = 0;
+        cnt[blockIdx.x * kCountPitch] = 0;
     }
 }
 
@@ -940,9 +941,9 @@ int4_topk_final_kernel(const void *in, uint64_t in_stride, uint32_t items, uint3
     __shared__ TopkLds s;
     const uint32_t tid = threadIdx.x, q = blockIdx.x;
     if (KIND == 2) {
-        items = cnt[q];
+        items = cnt[q * kCountPitch];
         if (items > cap) return;
-    } else if (cnt && cnt[q] <= cap)
+    } else if (cnt && cnt[q * kCountPitch] <= cap)
         return;
     const float *df = static_cast<const float *>(in) + (uint64_t)q * in_stride;
     const uint64_t *dl = static_cast<const uint64_t *>(in) + (uint64_t)q * in_stride;

@@ -524,8 +524,8 @@ cuddle_status cuddle_sharded_search_batch(cuddle_index *shard, cuddle_comm *comm
  * `device_id` (the caller's current device is left as it was), everything enqueued on `stream`, nothing
  * allocated, nothing copied to the host, nothing but kernels, so all of them may be recorded into a graph.
  * Work space is the caller's ([256-byte aligned], its size from the *_workspace call of the same sizes); it
- * holds nothing between calls, and two calls may share it only if they cannot overlap. Results are the same
- * bits from run to run. Arguments are checked before anything is enqueued. Row strides are in elements.
+ * holds nothing between calls, and two calls may share it only if they cannot overlap. Neither it nor an
+ * output may overlap an input or the other. Results are the same bits from run to run. Arguments are checked before anything is enqueued. Row strides are in elements.
  * An id outside [0, rows) (any negative one: padding) names no row: a lookup gives zeros for it, a gradient
  * leaves it out. dim <= 32768; fewer than 2^32 - 1 rows. */
 typedef enum cuddle_type { CUDDLE_TYPE_F32 = 0, CUDDLE_TYPE_F16 = 1, CUDDLE_TYPE_BF16 = 2 } cuddle_type;

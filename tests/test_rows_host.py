@@ -69,6 +69,7 @@ def test_query_refusals():
     assert L.cuddle_int4_workspace(32, 128, 2, 5, C.byref(need)) == _ffi.OK and need.value > 0
     assert L.cuddle_int4_workspace(32, 128, 2, 1025, C.byref(need)) == _ffi.ERR_UNSUPPORTED
     assert L.cuddle_int4_workspace(32, 128, 2, 5, None) == _ffi.ERR_BAD_ARG
+    assert L.cuddle_int4_workspace(10_000_000, 128, 0, 5, C.byref(need)) == _ffi.OK  # no queries: no work
     d = lambda r=_desc(), q=P, t=0, nq=5, m=0, out=P, w=ws, b=1 << 30: L.cuddle_int4_distances_device(  # noqa: E731
         None if r is None else C.byref(r), q, t, nq, m, out, w, b, 0, None)
     s = lambda r=_desc(), q=P, t=0, nq=2, k=5, m=0, i=P, o=P, w=ws, b=1 << 30: L.cuddle_int4_search_device(  # noqa: E731

@@ -3042,7 +3042,7 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
         // distribution of shape k), and the collection's room is not to run out by chance: odds under 1e-6 per query.
         // At most a sixteenth of the rows, but no fewer than expect half of that room to be filled.
         const uint64_t kn = (uint64_t)k * n;
-        const double least = std::sqrt((double)kn * (double)((qc + 255) / 256) / (0.24 * (double)qc));
+        const double nq_ = (double)std::max<uint64_t>(qc, 1), least = std::sqrt((double)kn * std::ceil(nq_ / 256) / (0.24 * nq_));
         const uint64_t expect = (uint64_t)std::min(std::max(least, 512.0), k == 1 ? 512.0 : k < 8 ? 1024.0 : 2048.0);
         const uint64_t rows = std::max<uint64_t>({4096, std::min<uint64_t>(kn / expect, n / 16), kn / (kTopChunk / 2)}), want = (rows + 15) / 16;
         if (qc * n >= kInt4SampleFrom && tiles / want >= 8) {
@@ -3490,6 +3490,27 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
     }
     uint8_t *ws = (uint8_t *)d_ws;
     const uint32_t t = (uint32_t)n_ids;
+    // Columns per lane: 16 bytes of the gradients where addresses and dim allow, one element otherwise. Lanes per chunk:
+    // the widest group that leaves few of its lanes without a column.
+    const uint32_t ts = type_size(type), os = type_size(grad_type), vmax = 16 / ts;
+    const bool vec = dim % vmax == 0 && aligned16(d_grad_out) && row_stride * ts % 16 == 0 && ((uintptr_t)d_grad & (std::min(vmax * os, 16u) - 1)) == 0;
+    const uint32_t V = vec ? vmax : 1, vpr = dim / V;
+    uint32_t lg = 6;
+    while (lg > 3 && ((vpr + (1u << lg) - 1) >> lg << lg) > vpr + vpr / 8) --lg;
+    GradArgs a{};
+    a.t = t;
+    a.chunks = w.chunks;
+    a.R = w.R;
+    a.lg = lg;
+    a.cbs = (vpr + (1u << lg) - 1) >> lg;
+    const uint64_t blocks = ((uint64_t)w.chunks * a.cbs + (256u >> lg) - 1) / (256u >> lg);
+    if (blocks > kMaxBlocksPerLaunch - 4096) return fail(CUDDLE_ERR_UNSUPPORTED, "n_ids * dim too large");
+    a.blocks = (uint32_t)blocks;
+    a.n_rows = n_rows;
+    a.dim = dim;
+    a.scale = scale;
+    a.accumulate = add ? 1u : 0u;
+    a.part = (float *)(ws + w.part);
     int cur = 0;
     uint8_t *named = nullptr;
     if (t <= kSortSmall) {
@@ -3533,28 +3554,7 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
         if (w.tile == 1024) sort(std::integral_constant<int, 4>{});
         else sort(std::integral_constant<int, 16>{});
     }
-    // Columns per lane: 16 bytes of the gradients where addresses and dim allow, one element otherwise. Lanes per chunk:
-    // the widest group that leaves few of its lanes without a column.
-    const uint32_t ts = type_size(type), os = type_size(grad_type), vmax = 16 / ts;
-    const bool vec = dim % vmax == 0 && aligned16(d_grad_out) && row_stride * ts % 16 == 0 && ((uintptr_t)d_grad & (std::min(vmax * os, 16u) - 1)) == 0;
-    const uint32_t V = vec ? vmax : 1, vpr = dim / V;
-    uint32_t lg = 6;
-    while (lg > 3 && ((vpr + (1u << lg) - 1) >> lg << lg) > vpr + vpr / 8) --lg;
-    GradArgs a;
     a.place = (const uint2 *)(ws + w.place[cur]);
-    a.t = t;
-    a.chunks = w.chunks;
-    a.R = w.R;
-    a.lg = lg;
-    a.cbs = (vpr + (1u << lg) - 1) >> lg;
-    const uint64_t blocks = ((uint64_t)w.chunks * a.cbs + (256u >> lg) - 1) / (256u >> lg);
-    if (blocks > kMaxBlocksPerLaunch - 4096) return fail(CUDDLE_ERR_UNSUPPORTED, "n_ids * dim too large");
-    a.blocks = (uint32_t)blocks;
-    a.n_rows = n_rows;
-    a.dim = dim;
-    a.scale = scale;
-    a.accumulate = add ? 1u : 0u;
-    a.part = (float *)(ws + w.part);
     a.named = named;
     const unsigned zero_blocks = named ? (unsigned)std::min<uint64_t>((grad_bytes + 16383) / 16384, 4096) : 0;
     with_type(type, [&](auto z) {

@@ -766,8 +766,9 @@ struct TopkLds {
 };
 
 // T and budget such that the k smallest (1 <= k <= C) of the keys key(0) .. key(C - 1) are those below T and `budget` of
-// those equal to T: T is the k-th smallest or, where nothing lies between, larger. 8 bits at a time from the highest bit in which the keys differ: distances share their leading bits, and a
-// histogram of those would be one counter that every thread adds to. All threads of a block of kTopThreads.
+// those equal to T: T is the k-th smallest or, where nothing lies between, larger. 8 bits at a time from the highest bit in
+// which the keys differ: distances share their leading bits, and a histogram of those would be one counter that every
+// thread adds to. All threads of a block of kTopThreads.
 template <class KeyFn>
 __device__ __forceinline__ void block_kth_key(uint32_t C, uint32_t k, KeyFn key, TopkLds &s, uint32_t &T, uint32_t &budget) {
     const uint32_t tid = threadIdx.x;
@@ -1090,8 +1091,9 @@ rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passe
 // More places: passes of up to 10 bits over tiles of J * 256 places, a count of the digits per tile (the first also clears
 // the map of rows that ids name, one byte each), then the scatter. Up to kSortSumTiles tiles a scatter's block adds the
 // counts up itself, beyond that a scan between the two does it. (Counting the next pass's digits in the scatter, by atomic
-// adds where the places land, measured slower: 64K skewed places 17 us for scatter and count, against 7 + 4.) J = 4 up to 256 K places (the tiles' waves rank their places one 64 after the other: 64K places 15 us with J = 16, 7
-// with 4), 16 beyond (the counts grow with the tiles).
+// adds where the places land, measured slower: 64K skewed places 17 us for scatter and count, against 7 + 4.) J = 4 up to
+// 256 K places (the tiles' waves rank their places one 64 after the other: 64K places 15 us with J = 16, 7 with 4), 16
+// beyond (the counts grow with the tiles).
 constexpr uint32_t kSortMaxBits = 10, kSortSumTiles = 64;
 
 template <int J, bool FIRST, class I>

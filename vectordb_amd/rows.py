@@ -8,7 +8,7 @@ no counterpart (its codes are 1-bit, its rows are fetched one at a time: src/sto
 
 The `*_device` calls take CUDA tensors, run on their device, enqueue on `stream` (default: torch's current stream of that
 device) and return tensors that are valid once that stream has been waited for. Work space comes from torch's
-allocator, on the same stream; a call may be recorded into a graph.
+allocator, on the same stream; a call may be recorded into a graph. Autograd records none of them.
 """
 from __future__ import annotations
 
@@ -239,7 +239,8 @@ def rows_grad_device(grad_out: torch.Tensor, ids: torch.Tensor, n_rows: int, sca
                      out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """Gradient of rows_lookup_device with respect to the table: row v = scale * the sum of grad_out [*ids.shape, dim] over
     the ids equal to v, summed in float32 in a fixed order: [n_rows, dim] of `dtype` (default: grad_out's).
-    out: a contiguous gradient [n_rows, dim] the sums are added to (rows without ids are not touched); returned."""
+    out: a contiguous gradient [n_rows, dim], apart from grad_out, that the sums are added to (rows without ids are not
+    touched); returned."""
     dim = grad_out.shape[-1]
     if tuple(grad_out.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"grad_out {tuple(grad_out.shape)} does not fit ids {tuple(ids.shape)}")

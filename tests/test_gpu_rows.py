@@ -107,6 +107,22 @@ def test_distances(gpu, n, d, nq, group, metric):
     assert np.all((np.abs(got - want) <= tol)[ok]), float((np.abs(got - want) / tol)[ok].max())
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,d,nq", [(300, 2100, 20), (270, 4100, 36), (520, 330, 20), (40, 1100, 100), (290, 190, 97), (5000, 130, 40), (17, 2500, 12)])
+def test_distances_many_queries(gpu, n, d, nq, group):
+    """Five and eight quartets of queries per pass, whole in LDS and in parts, odd last units, waves without rows."""
+    x, q = _rows(n, d, n + d), _rows(nq, d, n + d + 1)
+    r = R.int4_encode_device(x, group)
+    values = ref.encode(_np(x), group)[2]
+    want = ref.distances(values, _np(q), "l2")
+    got = _np(r.distances_device(q, "l2"))
+    ok = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), ~ok)
+    assert np.all((np.abs(got - want) <= ref.distance_tolerance(values, _np(q), want, "l2"))[ok])
+    for i in (0, nq // 2, nq - 1):  # a query's distances do not depend on its neighbours
+        assert np.array_equal(_np(r.distances_device(q[i:i + 1], "l2"))[0], got[i], equal_nan=True)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_distances_query_types(gpu, dtype):
     x, q = _rows(300, 192, 5), _rows(6, 192, 6, dtype)
@@ -477,6 +493,38 @@ def test_other_stream_and_graph(gpu):
         torch.cuda.synchronize()
         eager = step()
         assert all(torch.equal(a, b) for a, b in zip(held, eager)), turn
+
+
+def test_graph_of_large_calls(gpu):
+    """The sampled search (with and without an overflow of its collection) and the sort over many tiles, replayed."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(5)
+    n, t = 300_000, 70_000
+    x = torch.randn((n, 16), generator=gen, device="cuda")
+    r = R.int4_encode_device(x, 32)
+    q = torch.randn((128, 16), generator=gen, device="cuda")
+    g = torch.randn((t, 24), generator=gen, device="cuda")
+    ids = torch.randint(-5, 900, (t,), generator=gen, device="cuda")
+
+    def step():
+        return [*r.search_batch_device(q, 10), R.rows_grad_device(g, ids, n)]
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for turn in range(4):
+        q.mul_(1.25)
+        g.mul_(-1.5)
+        ids.copy_(torch.roll(ids, 3))
+        if turn == 2:
+            r.encode_device(x[:1].expand(n, 16).contiguous())  # every row the same: the collections overflow
+        if turn == 3:
+            r.encode_device(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step())), turn
+        if turn == 2:
+            assert torch.equal(held[0], torch.arange(10, device="cuda").expand(128, 10))
 
 
 def test_two_host_threads(gpu):

@@ -3539,7 +3539,7 @@ extern "C" cuddle_status cuddle_rows_grad_device(const void *d_grad_out, uint32_
                 auto pass = [&](auto hist_kernel, auto scatter_kernel, const void *src, unsigned extra, uint8_t *map) {
                     hipLaunchKernelGGL(hist_kernel, dim3(w.tiles + extra), dim3(256), 0, s, src, t, n_rows, shift, w.bits, w.tiles, hist, map);
                     if (scan) hipLaunchKernelGGL(rows_sort_scan_kernel, dim3(((1u << w.bits) + 63) / 64), dim3(1024), 0, s, hist, w.tiles, 1u << w.bits, total);
-                    hipLaunchKernelGGL(scatter_kernel, dim3(w.tiles), dim3(256), 0, s, src, t, n_rows, shift, w.bits, w.tiles, (const uint32_t *)hist,
+                    hipLaunchKernelGGL(scatter_kernel, dim3(w.tiles), dim3(1024), 0, s, src, t, n_rows, shift, w.bits, w.tiles, (const uint32_t *)hist,
                                        (const uint32_t *)(scan ? total : nullptr), out, map);
                 };
                 if (p == 0)

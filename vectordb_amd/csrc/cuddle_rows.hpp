@@ -1011,7 +1011,8 @@ rows_zero_kernel(void *p, uint64_t bytes) { zero_share(p, bytes, blockIdx.x, gri
 
 // Where 64 neighbouring keys of one wave go: off[digit] (LDS, this wave's own) holds the next place of each digit;
 // lanes with the same digit find each other by one ballot per digit bit, their order is the lane order.
-__device__ __forceinline__ uint32_t wave_rank(uint32_t d, bool in, uint32_t bits, uint32_t *off) {
+template <class C>
+__device__ __forceinline__ uint32_t wave_rank(uint32_t d, bool in, uint32_t bits, C *off) {
     uint64_t same = __ballot(in);
     for (uint32_t b = 0; b < bits; ++b) {
         const uint64_t m = __ballot((d >> b) & 1);
@@ -1022,7 +1023,7 @@ __device__ __forceinline__ uint32_t wave_rank(uint32_t d, bool in, uint32_t bits
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); // the reads above, before the update below
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (in && below == 0) off[d] += (uint32_t)__popcll(same);
+    if (in && below == 0) off[d] = (C)(off[d] + (uint32_t)__popcll(same));
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -1093,9 +1094,8 @@ rows_sort_small_kernel(const I *ids, uint32_t t, uint64_t n_rows, uint32_t passe
 // More places: passes of up to 10 bits over tiles of J * 256 places, a count of the digits per tile (the first also clears
 // the map of rows that ids name, one byte each), then the scatter. Up to kSortSumTiles tiles a scatter's block adds the
 // counts up itself, beyond that a scan between the two does it. (Counting the next pass's digits in the scatter, by atomic
-// adds where the places land, measured slower: 64K skewed places 17 us for scatter and count, against 7 + 4.) J = 4 up to
-// 256 K places (the tiles' waves rank their places one 64 after the other: 64K places 15 us with J = 16, 7 with 4), 16
-// beyond (the counts grow with the tiles).
+// adds where the places land, measured slower: 64K skewed places 17 us for scatter and count, against 6.5 + 3.5.) J = 4 up to
+// 256 K places (more blocks, shorter chains of ranks), 16 beyond (the counts grow with the tiles).
 constexpr uint32_t kSortMaxBits = 10, kSortSumTiles = 64;
 
 template <int J, bool FIRST, class I>
@@ -1152,68 +1152,80 @@ rows_sort_scan_kernel(uint32_t *hist, uint32_t tiles, uint32_t bins, uint32_t *t
     }
 }
 
-// total == nullptr: hist holds plain counts, to be added up here.
+// total == nullptr: hist holds plain counts, to be added up here. Sixteen waves: the ranking is a chain per wave, and a
+// block's start waits for the counts (64K places: 6.5 us, 8.2 with four waves; 1M: 15 to 20, and 20 to 24). Block 1024, a
+// wave has J / 4 times 64 neighbouring places.
 template <int J, bool FIRST, class I>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 rows_sort_scatter_kernel(const void *src, uint32_t t, uint64_t n_rows, uint32_t shift, uint32_t bits, uint32_t tiles, const uint32_t *hist, const uint32_t *total,
                          uint2 *out, uint8_t *named) {
-    __shared__ uint32_t off[4][1u << kSortMaxBits];
+    constexpr int W = 16, K = J * 4 / W;
+    __shared__ __attribute__((aligned(4))) uint16_t off[W][1u << kSortMaxBits]; // a wave's next place of the digit, from the tile's first
     __shared__ uint32_t tot[(1u << kSortMaxBits) + 1];
     __shared__ uint32_t before[1u << kSortMaxBits]; // places of the digit in the tiles before
     const uint32_t tid = threadIdx.x, w = tid >> 6, lane = tid & 63, bins = 1u << bits;
-    for (uint32_t i = tid; i < bins; i += 256) {
-        off[0][i] = off[1][i] = off[2][i] = off[3][i] = 0;
-        if (total) {
-            tot[i] = total[i];
-            before[i] = hist[(uint64_t)blockIdx.x * bins + i];
-        } else {
-            uint32_t all = 0, bef = 0;
-#pragma unroll 16
-            for (uint32_t u = 0; u < tiles; ++u) {
-                const uint32_t v = hist[(uint64_t)u * bins + i];
-                all += v;
-                bef += u < blockIdx.x ? v : 0u;
-            }
-            tot[i] = all;
-            before[i] = bef;
-        }
-    }
-    __syncthreads();
-    const uint32_t b = blockIdx.x * (J * 256) + w * (J * 64);
-    uint32_t k[J], ps[J];
+    uint32_t k[K], ps[K];
+    const uint32_t b = blockIdx.x * (J * 256) + w * (K * 64);
 #pragma unroll
-    for (uint32_t j = 0; j < J; ++j) {
+    for (int j = 0; j < K; ++j) { // on their way while the counts are added up
         const uint32_t i = b + j * 64 + lane;
-        const bool in = i < t;
         k[j] = ps[j] = 0u;
-        if (in && FIRST) {
+        if (i < t && FIRST) {
             k[j] = grad_key(static_cast<const I *>(src), i, n_rows);
             ps[j] = i;
-        } else if (in) {
+        } else if (i < t) {
             const uint2 e = static_cast<const uint2 *>(src)[i];
             k[j] = e.x;
             ps[j] = e.y;
         }
-        if (in) atomicAdd(&off[w][(k[j] >> shift) & (bins - 1)], 1u);
+    }
+    for (uint32_t i = tid; i < bins; i += 1024) {
+        tot[i] = total ? total[i] : 0u;
+        before[i] = total ? hist[(uint64_t)blockIdx.x * bins + i] : 0u;
+    }
+    for (uint32_t i = tid; i < W << bits; i += 1024) off[i >> bits][i & (bins - 1)] = 0;
+    __syncthreads();
+    if (!total) { // 1024 / bins threads per digit, a share of the tiles each
+        const uint32_t i = tid & (bins - 1), step = 1024u >> bits;
+        uint32_t all = 0, bef = 0;
+        for (uint32_t u0 = tid >> bits; u0 < tiles; u0 += 16 * step) { // sixteen reads in flight
+            uint32_t v[16];
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) v[j] = u0 + j * step < tiles ? hist[(uint64_t)(u0 + j * step) * bins + i] : 0u;
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) {
+                all += v[j];
+                bef += u0 + j * step < blockIdx.x ? v[j] : 0u;
+            }
+        }
+        if (all) atomicAdd(&tot[i], all);
+        if (bef) atomicAdd(&before[i], bef);
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) { // the wave's own counts
+        const bool in = b + j * 64 + lane < t;
+        const uint32_t d = (k[j] >> shift) & (bins - 1);
+        if (in) atomicAdd(reinterpret_cast<uint32_t *>(off[w]) + (d >> 1), 1u << (16 * (d & 1))); // a half: 64 K counts at most
         if (FIRST && named && in && k[j] < n_rows) named[k[j]] = 1;
     }
-    wave0_exclusive_scan_lds(tot, bins);
     __syncthreads();
-    for (uint32_t i = tid; i < bins; i += 256) {
-        uint32_t run = tot[i] + before[i];
+    wave0_exclusive_scan_lds(tot, bins);
+    for (uint32_t i = tid; i < bins; i += 1024) {
+        uint32_t run = 0;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
+        for (int v = 0; v < W; ++v) {
             const uint32_t c = off[v][i];
-            off[v][i] = run;
+            off[v][i] = (uint16_t)run;
             run += c;
         }
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t j = 0; j < J; ++j) {
+    for (int j = 0; j < K; ++j) {
+        const uint32_t d = (k[j] >> shift) & (bins - 1);
         const bool in = b + j * 64 + lane < t;
-        const uint32_t at = wave_rank((k[j] >> shift) & (bins - 1), in, bits, off[w]);
-        if (in) out[at] = make_uint2(k[j], ps[j]);
+        const uint32_t at = wave_rank(d, in, bits, off[w]);
+        if (in) out[tot[d] + before[d] + at] = make_uint2(k[j], ps[j]);
     }
 }
 

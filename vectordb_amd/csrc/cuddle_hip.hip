@@ -3002,17 +3002,6 @@ constexpr uint64_t kInt4MaxRound = 32768;          // queries per round (the lau
 // launches cost about 30 us).
 constexpr uint64_t kInt4SampleFrom = 32ull << 20;
 
-// Items per block of a selection level: fewer where that fills the chip sooner (50 000 items, one query, k = 100: 16 us in 7
-// blocks, 6 in 25), as long as one more level answers and a chunk is several times what it keeps.
-uint32_t top_chunk(uint64_t items, uint32_t nq, uint32_t k) {
-    const uint64_t fits = 3072 / k; // parts that the last level takes without becoming the longer one
-    for (uint32_t chunk : {1024u, 2048u, 4096u}) {
-        const uint64_t parts = (items + chunk - 1) / chunk;
-        if (chunk >= 8 * k && parts <= fits && parts * nq <= 1024) return chunk;
-    }
-    return kTopChunk;
-}
-
 Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
     Int4Ws w;
     uint64_t qc = std::min<uint64_t>(nq, kInt4MaxRound);

@@ -1,0 +1,81 @@
+"""GPU: the embedding table's C entry points on arrays that lie tightly between guard bytes, at the sizes where a list or an
+array ends inside what a kernel handles at a time."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from vectordb_amd import _ffi
+from vectordb_amd import rows as R
+
+pytestmark = pytest.mark.gpu
+
+GUARD, MARK = 16384, 0xA5
+
+
+class Carver:
+    """Arrays out of one allocation, 256-byte aligned, GUARD marked bytes behind each one's last byte."""
+
+    def __init__(self, gpu, room):
+        self.buf = torch.full((room,), MARK, dtype=torch.uint8, device=torch.device("cuda", gpu))
+        self.at, self.spans = 0, []
+
+    def take(self, shape, dtype):
+        size = int(np.prod(shape)) * torch.empty((), dtype=dtype).element_size()
+        a = self.at
+        self.spans.append((a, a + size))
+        self.at = (a + size + GUARD + 255) // 256 * 256
+        assert self.at <= self.buf.numel()
+        return self.buf[a:a + size].view(dtype).view(shape)
+
+    def check(self):
+        torch.cuda.synchronize()
+        for _, end in self.spans:
+            assert bool((self.buf[end:end + GUARD] == MARK).all()), f"written behind byte {end}"
+
+
+def _search(gpu, x, q, k, group=32):
+    """cuddle_int4_search_device on tight arrays: (ids, dist, the table)."""
+    n, dim = x.shape
+    nq = q.shape[0]
+    code_bytes, stride = R.Int4Rows._sizes(n, dim, group)
+    need = C.c_uint64(0)
+    _ffi.check(_ffi.lib().cuddle_int4_workspace(n, dim, nq, k, C.byref(need)))
+    sizes = [code_bytes, 2 * n * stride, 8 * n, 4 * nq * dim, 8 * nq * k, 4 * nq * k, 4 * nq, need.value]
+    c = Carver(gpu, sum(s + GUARD + 256 for s in sizes))
+    table = R.Int4Rows(c.take((code_bytes,), torch.uint8), c.take((n, stride), torch.bfloat16), c.take((n,), torch.float64), n, dim, group)
+    table.encode_device(x)
+    qt = c.take((nq, dim), torch.float32)
+    qt.copy_(q)
+    ids, dist, count = c.take((nq, k), torch.int64), c.take((nq, k), torch.float32), c.take((nq,), torch.int32)
+    ws = c.take((need.value,), torch.uint8)
+    _ffi.check(_ffi.lib().cuddle_int4_search_device(C.byref(table._desc), qt.data_ptr(), _ffi.TYPE_F32, nq, k, _ffi.METRIC_L2, ids.data_ptr(), dist.data_ptr(),
+                                                    count.data_ptr(), ws.data_ptr(), need.value, gpu, torch.cuda.current_stream().cuda_stream))
+    c.check()
+    assert count.tolist() == [min(k, n)] * nq
+    return ids, dist, table
+
+
+# second-level chunks that are longer than k and hold fewer than k rows (the rest is fill): 908 of 1808, 64 of 108,
+# 47 of 124, 36 of 208
+@pytest.mark.parametrize("n,nq,k", [(73_828, 1, 1000), (73_828, 3, 1000), (671_800, 1, 100), (671_800, 2, 100), (876_545, 2, 77), (335_900, 4, 200)])
+def test_search_with_short_last_lists(gpu, n, nq, k):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(n + nq)
+    x = torch.randn((n, 16), generator=gen, device="cuda")
+    q = torch.randn((nq, 16), generator=gen, device="cuda")
+    ids, dist, table = _search(gpu, x, q, k)
+    d = table.distances_device(q)
+    order = torch.argsort(d, dim=1, stable=True)[:, :k]
+    assert torch.equal(ids, order)
+    assert torch.equal(dist, torch.gather(d, 1, order))
+
+
+def test_search_with_short_last_lists_after_an_overflow(gpu):
+    """A sampled search whose collections all overflow (every row the same): the levels answer, with such a last list."""
+    n, nq, k = 335_900, 100, 200
+    x = torch.ones((n, 16), device="cuda")
+    ids, dist, table = _search(gpu, x, torch.zeros((nq, 16), device="cuda"), k)
+    assert torch.equal(ids, torch.arange(k, device="cuda").expand(nq, k))
+    assert bool((dist == dist[0, 0]).all()) and abs(float(dist[0, 0]) - 16) < 0.1

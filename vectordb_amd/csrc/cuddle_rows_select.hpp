@@ -109,7 +109,9 @@ __device__ __forceinline__ void block_kth_key(uint32_t C, uint32_t k, KeyFn key,
 }
 
 // The k smallest of C items with keys keys[i] (LDS) and item(i) = key << 32 | row: emit(place, item) in any order, places
-// 0 .. min(k, C) - 1. Of the items equal to the last key the lowest rows. s.n is zero on entry. All threads of the block.
+// from 0 on. Of the items equal to the last key the lowest rows. Fill (~0) is never handed on: it has one row number for
+// all, so among the k smallest - where fewer than k real items are left - no row would tell apart how many of it are
+// wanted. s.n is zero on entry and counts what was emitted, at most k. All threads of the block.
 template <class ItemFn, class EmitFn>
 __device__ __forceinline__ void block_smallest(const uint32_t *keys, uint32_t C, uint32_t k, ItemFn item, EmitFn emit, TopkLds &s) {
     const uint32_t tid = threadIdx.x;
@@ -131,7 +133,7 @@ __device__ __forceinline__ void block_smallest(const uint32_t *keys, uint32_t C,
     for (uint32_t i = tid; i < C; i += kTopThreads) {
         if (keys[i] > T) continue;
         const uint64_t v = item(i);
-        if (keys[i] < T || (uint32_t)v <= R) emit(atomicAdd(&s.n, 1u), v);
+        if (v != ~0ull && (keys[i] < T || (uint32_t)v <= R)) emit(atomicAdd(&s.n, 1u), v);
     }
 }
 
@@ -160,7 +162,8 @@ int4_topk_level_kernel(const void *in, uint64_t in_stride, uint64_t items, uint3
         block_smallest(
             keys, C, k, [&](uint32_t i) -> uint64_t { return FIRST ? (uint64_t)keys[i] << 32 | (uint32_t)(base + i) : dl[i]; },
             [&](uint32_t at, uint64_t v) { o[at] = v; }, s);
-        for (uint32_t i = C + tid; i < k; i += kTopThreads) o[i] = ~0ull;
+        __syncthreads();
+        for (uint32_t i = s.n + tid; i < k; i += kTopThreads) o[i] = ~0ull;
     }
 }
 

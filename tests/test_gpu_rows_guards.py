@@ -9,6 +9,8 @@ import torch
 from vectordb_amd import _ffi
 from vectordb_amd import rows as R
 
+import rows_reference as ref
+
 pytestmark = pytest.mark.gpu
 
 GUARD, MARK = 16384, 0xA5
@@ -79,3 +81,25 @@ def test_search_with_short_last_lists_after_an_overflow(gpu):
     ids, dist, table = _search(gpu, x, torch.zeros((nq, 16), device="cuda"), k)
     assert torch.equal(ids, torch.arange(k, device="cuda").expand(nq, k))
     assert bool((dist == dist[0, 0]).all()) and abs(float(dist[0, 0]) - 16) < 0.1
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,dim,nq", [(256, 64, 24), (4096, 128, 32), (513, 16, 61), (1024, 100, 128), (16, 65, 88), (1, 128, 101), (2048, 33, 200)])
+def test_distances_of_short_rows(gpu, n, dim, nq, group):
+    """Eight quartets of queries against rows of one or two units, the scales' last row at the array's end."""
+    rng = np.random.default_rng(n + dim + nq)
+    x = torch.from_numpy(rng.standard_normal((n, dim)).astype(np.float32)).cuda(gpu)
+    q = torch.from_numpy(rng.standard_normal((nq, dim)).astype(np.float32)).cuda(gpu)
+    code_bytes, stride = R.Int4Rows._sizes(n, dim, group)
+    need = C.c_uint64(0)
+    _ffi.check(_ffi.lib().cuddle_int4_workspace(n, dim, nq, 0, C.byref(need)))
+    c = Carver(gpu, code_bytes + 2 * n * stride + 8 * n + 4 * n * nq + need.value + 5 * (GUARD + 256))
+    table = R.Int4Rows(c.take((code_bytes,), torch.uint8), c.take((n, stride), torch.bfloat16), c.take((n,), torch.float64), n, dim, group)
+    table.encode_device(x)
+    out, ws = c.take((nq, n), torch.float32), c.take((need.value,), torch.uint8)
+    _ffi.check(_ffi.lib().cuddle_int4_distances_device(C.byref(table._desc), q.data_ptr(), _ffi.TYPE_F32, nq, _ffi.METRIC_L2, out.data_ptr(), ws.data_ptr(),
+                                                       need.value, gpu, torch.cuda.current_stream().cuda_stream))
+    c.check()
+    values = ref.encode(x.cpu().numpy(), group)[2]
+    want = ref.distances(values, q.cpu().numpy(), "l2")
+    assert np.all(np.abs(out.cpu().double().numpy() - want) <= ref.distance_tolerance(values, q.cpu().numpy(), want, "l2"))

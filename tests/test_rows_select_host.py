@@ -25,3 +25,11 @@ def program(tmp_path_factory):
 def test_selection_on_the_host(program, n, k, nq, kind):
     r = subprocess.run([program, str(n), str(k), str(nq), kind], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_no_launch_reads_behind_the_scales(tmp_path):
+    exe = str(tmp_path / "plan_on_host")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-I", os.path.join(ROOT, "vectordb_amd", "csrc"), os.path.join(ROOT, "tests", "cpp", "plan_on_host.cpp"),
+                    "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr

@@ -2983,11 +2983,6 @@ template <class F> void with_id(uint32_t bits, F f) {
 constexpr size_t kAlign = 256;
 size_t round_ws(size_t b) { return (b + kAlign - 1) & ~(kAlign - 1); }
 
-constexpr uint32_t int4_lds_kb(int qt) { return qt >= 5 ? 128u : qt >= 3 ? 144u : 64u; } // digits per block: one large block per CU, or several
-// Up to four queries whose digits fit a block's LDS: the distance kernel makes them itself. A round of a call is fused if
-// its queries are this few, so a call of more queries lays out room for digits also for a last, smaller round.
-bool int4_fused(uint64_t nq, uint32_t dim) { return nq <= 4 && (int4_units(dim) + 7) / 8 * 8 <= int4_lds_kb(1); }
-
 // Work space of the distance and search calls: the queries' digits, and for a search the distances of `qc` queries and
 // two selection buffers.
 struct Int4Ws {
@@ -3046,16 +3041,9 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
     return w;
 }
 
-// Launch shapes of the distance kernel. One quartet of queries: codes are the bound, so many of them are requested at a
-// time (four pieces of 1 KB per wave). More: QT quartets per wave, the count among those built that costs least.
-// A wave's pass over its codes unpacks them once and multiplies them QT times; unpacking, addresses and the wait cost
-// about as much as three quartets' products (1M x 960, one pass: 140 us with 5 quartets, 190 with 8, 114 with 4, 98 with
-// 3). 20 queries: 161 us with 5, 210 with 8; 64: 401 with 8, 498 with 5, 471 with 4; 100: 682 with 5, 730 with 8, 779
-// with 4. Six and seven quartets were built and won nowhere by more than 4 %. Digits that do not fit the block's LDS at
-// once are fetched anew for every 256 rows, from the L2, and change nothing in the order (100k x 4096, 64 queries: 221 us
-// with 8, 264 with 5, 289 with 4).
 template <int G, int QT, int T, int P, bool FUSED, bool NT, class TQ>
-void int4_launch(Int4DistArgs a, hipStream_t s) {
+cuddle_status int4_launch(Int4DistArgs a, hipStream_t s) {
+    if (a.gs % int4_scales(P, G)) return fail(CUDDLE_ERR_UNSUPPORTED, "rows of %u scales for a kernel that reads %u at a time", a.gs, int4_scales(P, G));
     constexpr uint32_t NW = int4_block(QT, T) / 64;
     a.ku = std::min<uint32_t>((a.units + P - 1) / P * P, int4_lds_kb(QT) / QT / P * P);
     a.ys = ((a.nq + 3) / 4 + QT - 1) / QT;
@@ -3089,46 +3077,33 @@ void int4_launch(Int4DistArgs a, hipStream_t s) {
     if (a.ys > 1) xs = (xs + 7) / 8 * 8;
     a.xs = (uint32_t)xs;
     hipLaunchKernelGGL((int4_distance_kernel<G, QT, T, P, FUSED, NT, TQ>), dim3((unsigned)(a.xs * a.ys)), dim3(int4_block(QT, T)), lds, s, a);
+    HIP_TRY(hipGetLastError());
+    return CUDDLE_OK;
 }
 
 template <int G>
-void int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStream_t s) {
-    const uint32_t quads = (a.nq + 3) / 4;
-    const bool few_units = a.units < 6; // short rows: more tiles and fewer units at a time
+cuddle_status int4_launch_group(const Int4DistArgs &a, uint32_t type, bool fused, hipStream_t s) {
+    const Int4Shape shape = int4_shape(a.units, a.nq, fused);
+    cuddle_status st = CUDDLE_OK;
     if (fused) {
         with_type(type, [&](auto z) {
             using TQ = decltype(z);
             // beyond the Infinity Cache (256 MB) nothing of the codes is left for the next call
             const bool nt = (a.n + 15) / 16 * a.units * kInt4UnitBytes > (256ull << 20) && !a.stride;
-            if (few_units && nt) int4_launch<G, 1, 4, 2, true, true, TQ>(a, s);
-            else if (few_units) int4_launch<G, 1, 4, 2, true, false, TQ>(a, s);
-            else if (nt) int4_launch<G, 1, 2, 4, true, true, TQ>(a, s);
-            else int4_launch<G, 1, 2, 4, true, false, TQ>(a, s);
+            if (shape.p == 2 && nt) st = int4_launch<G, 1, 4, 2, true, true, TQ>(a, s);
+            else if (shape.p == 2) st = int4_launch<G, 1, 4, 2, true, false, TQ>(a, s);
+            else if (nt) st = int4_launch<G, 1, 2, 4, true, true, TQ>(a, s);
+            else st = int4_launch<G, 1, 2, 4, true, false, TQ>(a, s);
         });
-        return;
+        return st;
     }
-    uint32_t best = 1, cost = ~0u; // (of equal costs the larger: its codes are unpacked less often)
-    for (uint32_t qt : {1u, 2u, 3u, 4u, 5u, 8u}) {
-        const uint32_t c = (quads + qt - 1) / qt * (qt + 3);
-        if (c <= cost) {
-            cost = c;
-            best = qt;
-        }
-    }
-    switch (best) {
-    case 1: int4_launch<G, 1, 4, 2, false, false, float>(a, s); break;
-    case 2: int4_launch<G, 2, 2, 2, false, false, float>(a, s); break;
-    case 3: int4_launch<G, 3, 2, 2, false, false, float>(a, s); break;
-    case 4: int4_launch<G, 4, 2, 2, false, false, float>(a, s); break;
-    case 5:
-        // rows of one or two units: a pair of units is all there is to request ahead, and two tiles keep the wave busy
-        // (1M x 128, 100 queries: 245 us against 295; from 192 dimensions on equal or slower, 100k x 4096: 455 against 345)
-        if (a.units < 3) int4_launch<G, 5, 2, 2, false, false, float>(a, s);
-        else int4_launch<G, 5, 1, 4, false, false, float>(a, s);
-        break;
-    default:
-        int4_launch<G, 8, 1, 4, false, false, float>(a, s);
-        break;
+    switch (shape.qt) {
+    case 1: return int4_launch<G, 1, 4, 2, false, false, float>(a, s);
+    case 2: return int4_launch<G, 2, 2, 2, false, false, float>(a, s);
+    case 3: return int4_launch<G, 3, 2, 2, false, false, float>(a, s);
+    case 4: return int4_launch<G, 4, 2, 2, false, false, float>(a, s);
+    case 5: return shape.p == 2 ? int4_launch<G, 5, 2, 2, false, false, float>(a, s) : int4_launch<G, 5, 1, 4, false, false, float>(a, s);
+    default: return shape.p == 2 ? int4_launch<G, 8, 1, 2, false, false, float>(a, s) : int4_launch<G, 8, 1, 4, false, false, float>(a, s);
     }
 }
 
@@ -3160,10 +3135,10 @@ Int4DistArgs int4_prepare(const cuddle_int4_rows *r, const void *queries, uint32
     return a;
 }
 
-void int4_run(const Int4DistArgs &a, uint32_t group, uint32_t type, bool fused, hipStream_t s) {
-    if (group == 32) int4_launch_group<32>(a, type, fused, s);
-    else if (group == 64) int4_launch_group<64>(a, type, fused, s);
-    else int4_launch_group<128>(a, type, fused, s);
+cuddle_status int4_run(const Int4DistArgs &a, uint32_t group, uint32_t type, bool fused, hipStream_t s) {
+    if (group == 32) return int4_launch_group<32>(a, type, fused, s);
+    if (group == 64) return int4_launch_group<64>(a, type, fused, s);
+    return int4_launch_group<128>(a, type, fused, s);
 }
 
 cuddle_status check_query_call(const cuddle_int4_rows *r, const void *queries, uint32_t type, uint32_t nq, uint32_t metric) {
@@ -3278,7 +3253,7 @@ extern "C" cuddle_status cuddle_int4_distances_device(const cuddle_int4_rows *ro
         Int4DistArgs a = int4_prepare(rows, d_queries, type, q0, std::min(w.qc, n_queries - q0), metric, (uint8_t *)d_ws, w, fused, (hipStream_t)stream_);
         a.dist = d_dist + (uint64_t)q0 * rows->n;
         a.dstride = rows->n;
-        int4_run(a, rows->group, type, fused, (hipStream_t)stream_);
+        ST_TRY(int4_run(a, rows->group, type, fused, (hipStream_t)stream_));
         HIP_TRY(hipGetLastError());
     }
     return CUDDLE_OK;
@@ -3322,7 +3297,7 @@ extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows,
             a.dstride = w.stiles * 16;
             a.stride = w.stride;
             a.stiles = w.stiles;
-            int4_run(a, rows->group, type, fused, s);
+            ST_TRY(int4_run(a, rows->group, type, fused, s));
             const uint32_t items = (uint32_t)(w.stiles * 16), in_lds = items <= (36u << 10) ? 1u : 0u;
             static std::once_flag once[kMaxDevices];
             std::call_once(once[device_id & (kMaxDevices - 1)], [] {
@@ -3334,7 +3309,7 @@ extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows,
             a.cnt = cnt;
             a.list = (uint64_t *)(ws + w.list);
             a.cap = kTopChunk;
-            int4_run(a, rows->group, type, fused, s);
+            ST_TRY(int4_run(a, rows->group, type, fused, s));
             hipLaunchKernelGGL(int4_topk_final_kernel<2>, dim3(nq), dim3(kTopThreads), 0, s, (const void *)a.list, (uint64_t)kTopChunk, 0u, k, found, (const uint32_t *)cnt,
                                kTopChunk, ids, od, oc);
         }
@@ -3343,7 +3318,7 @@ extern "C" cuddle_status cuddle_int4_search_device(const cuddle_int4_rows *rows,
         a.dstride = rows->n;
         a.redo = cnt;
         a.cap = kTopChunk;
-        int4_run(a, rows->group, type, fused, s);
+        ST_TRY(int4_run(a, rows->group, type, fused, s));
         const void *in = dist;
         uint64_t stride = rows->n, items = rows->n;
         int level = 0;

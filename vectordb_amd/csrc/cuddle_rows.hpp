@@ -21,6 +21,7 @@
 #pragma once
 
 #include "cuddle_kernels.hpp"
+#include "cuddle_rows_plan.hpp"
 #include "cuddle_rows_select.hpp"
 
 namespace cuddle {
@@ -28,19 +29,10 @@ namespace cuddle {
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2;
-constexpr uint32_t kInt4Unit = 64;      // components per unit
-constexpr uint32_t kInt4UnitBytes = 512; // 16 rows x 32 bytes
-
 // Offset in a tile of byte b = 8h + i of row r's unit u.
 __device__ __forceinline__ uint32_t int4_code_at(uint32_t units, uint32_t u, uint32_t r, uint32_t b) {
     if (u == units - 1 && !(u & 1)) return u * kInt4UnitBytes + r * 32 + b;
     return (u >> 1) * (2 * kInt4UnitBytes) + r * 64 + (b >> 3) * 16 + (u & 1) * 8 + (b & 7);
-}
-
-__host__ __device__ __forceinline__ uint32_t int4_units(uint32_t dim) { return (dim + kInt4Unit - 1) / kInt4Unit; }
-__host__ __device__ __forceinline__ uint32_t int4_gstride(uint32_t dim, uint32_t group) {
-    const uint32_t groups = (dim + group - 1) / group, m = groups > 4 ? 8 : groups > 2 || group == 32 ? 4 : 2;
-    return (groups + m - 1) / m * m;
 }
 
 // ---- element types ---------------------------------------------------------------------------
@@ -442,10 +434,6 @@ __device__ __forceinline__ double int4_add(double acc, i32x4_t c, double s) {
     return __builtin_fma(s, __builtin_fma((double)(c[2] + (c[3] << 8)), 65536.0, (double)(c[0] + (c[1] << 8))), acc);
 }
 
-// Threads. Five and eight quartets of one tile: sixteen waves around one copy of the digits (1M x 960, 64 queries: 472 us,
-// 496 with eight waves of two tiles each; 20 queries: 196 and 215).
-__host__ __device__ constexpr int int4_block(int qt, int t) { return qt >= 5 && t == 1 ? 1024 : qt >= 3 ? 512 : 256; }
-
 struct Int4DistArgs {
     const uint8_t *codes;
     const uint16_t *scales;
@@ -603,7 +591,7 @@ int4_distance_kernel(Int4DistArgs a) {
             s_test[tid] = y * QT * 4 + tid < a.nq ? int4_test(a.metric, s_tau[tid], s_info[tid]) : Int4Test{0.f, -__builtin_huge_valf()};
         __syncthreads();
     }
-    constexpr int SC = P * 64 / G; // scales
+    constexpr int SC = int4_scales(P, G);
     struct Piece {
         uint2 w[T][P];
         Pack<uint16_t, SC> sc[T];
@@ -625,7 +613,7 @@ int4_distance_kernel(Int4DistArgs a) {
                 v.w[t][p] = make_uint2(b[0], b[1]);
                 v.w[t][p + 1] = make_uint2(b[2], b[3]);
             }
-            v.sc[t] = *reinterpret_cast<const Pack<uint16_t, SC> *>(sp + 2 * (ub * 64 / G) + so); // gs is a multiple of SC: these are the row's own
+            v.sc[t] = *reinterpret_cast<const Pack<uint16_t, SC> *>(sp + 2 * (ub * 64 / G) + so); // gs is a multiple of SC (checked at the launch): these are the row's own
         }
     };
     // The next piece is on its way while this one is worked on. Few queries from a cache: the waves cover for each other

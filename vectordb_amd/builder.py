@@ -322,6 +322,11 @@ def build_index(vectors, branching_factor: int = 100, target_leaf_size: int = 10
     assert x.dim() == 2 and x.shape[0] > 0
     dev = torch.device(device) if device is not None else x.device
     x = x.to(device=dev, dtype=torch.float32)
+    rows = x
+    if x.is_cuda:
+        from .rows import _rows2d
+
+        rows = _rows2d(x)  # a transposed tensor is copied once here, not whole at every lookup
     n, d = x.shape
     gen = torch.Generator(device="cpu")  # scalar draws only; the heavy math runs on `dev`
     gen.manual_seed(seed)
@@ -330,7 +335,7 @@ def build_index(vectors, branching_factor: int = 100, target_leaf_size: int = 10
     old = sys.getrecursionlimit()
     sys.setrecursionlimit(max(old, 10000))
     try:
-        roots = _build_recursive(tree, x, torch.arange(n, device=dev), 0, target_leaf_size, branching_factor, m,
+        roots = _build_recursive(tree, rows, torch.arange(n, device=dev), 0, target_leaf_size, branching_factor, m,
                                  max_iterations, gen)
     finally:
         sys.setrecursionlimit(old)
@@ -348,7 +353,7 @@ def build_index(vectors, branching_factor: int = 100, target_leaf_size: int = 10
         if cnt:
             order.append(tree.vec[i])
     ids_t = torch.cat(order) if order else torch.zeros(0, dtype=torch.long, device=dev)
-    stored = _take(x, ids_t)
+    stored = _take(rows, ids_t)
     vec_lc = stored.cpu().numpy()
     fi = FlatIndex(
         dim=d, metric=m, code_kind=_ffi.CODE_BINARY if code_kind == "binary" else _ffi.CODE_RABITQ,

@@ -43,3 +43,13 @@ def test_strided_rows_are_copied_once(gpu, monkeypatch, layout):
     _same(build_index(given, 8, 30, "l2", 10, seed=2, threshold=0.0, device="cuda"), want)
     assert len(tables) > 10 and len(set(tables)) == 1 and tables[0][1][1] == 1  # one table, whole rows
     assert (tables[0][0] == given.data_ptr()) if layout == "part of wider rows" else (tables[0][1][0] == 24)  # a copy only where needed
+
+
+def test_rows_longer_than_a_lookup_takes(gpu):
+    """A single leaf needs no assignment, whose dimensions are limited too."""
+    x = clustered(12, 33_000, 3, 6)
+    want = build_index(x, 8, 30, "l2", 10, seed=2, threshold=0.0)
+    got = build_index(torch.from_numpy(x).cuda(gpu), 8, 30, "l2", 10, seed=2, threshold=0.0)
+    assert np.array_equal(got.vectors, want.vectors) and np.array_equal(got.codes, want.codes) and np.array_equal(got.ids, want.ids)
+    # a mean of 12 floats in two orders: 11 roundings of sums each, and one of the quotient
+    assert np.all(np.abs(got.centroids - want.centroids) <= (2 * 11 + 2) * 2.0 ** -24 * np.abs(x).sum(0) / 12)

@@ -197,8 +197,9 @@ def _kmeans_fit_native(x: torch.Tensor, k: int, metric: int, max_iterations: int
 
 
 def _take(x: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
-    """Rows of x by index; on the GPU through the library (rows_lookup_device: the same values)."""
-    if not x.is_cuda:
+    """Rows of x by index; on the GPU through the library (rows_lookup_device: the same values), up to the 32768
+    components that its kernels take."""
+    if not x.is_cuda or x.shape[1] > 32768:
         return x[idx]
     from .rows import rows_lookup_device
 

@@ -8,7 +8,9 @@ no counterpart (its codes are 1-bit, its rows are fetched one at a time: src/sto
 
 The `*_device` calls take CUDA tensors, run on their device, enqueue on `stream` (default: torch's current stream of that
 device) and return tensors that are valid once that stream has been waited for. Work space comes from torch's
-allocator, on the same stream; a call may be recorded into a graph. Autograd records none of them.
+allocator, on the same stream; a call may be recorded into a graph. Autograd records none of them, so a call whose result
+is a smooth function of an input (a lookup's table, the queries of distances, a gradient) refuses one that requires a
+gradient outside `torch.no_grad()`: detach it and call `rows_grad_device`.
 """
 from __future__ import annotations
 
@@ -40,6 +42,12 @@ def _cuda(*tensors: torch.Tensor) -> torch.device:
         if t.device != dev:
             raise ValueError(f"tensors on {dev} and {t.device}")
     return dev
+
+
+def _no_grad(what: str, t: torch.Tensor) -> None:
+    """Refuses an input whose gradient would be lost without a word: no call here is recorded by autograd."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, which autograd does not record here: pass {what}.detach()")
 
 
 def _rows2d(x: torch.Tensor) -> torch.Tensor:
@@ -171,6 +179,7 @@ class Int4Rows:
     def distances_device(self, queries: torch.Tensor, metric="l2", stream=None) -> torch.Tensor:
         """distance(query, row) of queries [nq, dim] (float32, float16, bfloat16) to every row: float32 [nq, n]."""
         (dev, kind), m = self._queries(queries), metric_id(metric)
+        _no_grad("queries", queries)
         ctx, index, st = _enter(dev, stream, queries, *self._arrays)
         with ctx:
             q = queries.contiguous()
@@ -224,6 +233,7 @@ def rows_lookup_device(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.
     any shape: [*ids.shape, dim] of the table's type. An id outside [0, n) gives zeros."""
     if table.dim() != 2:
         raise ValueError(f"rows must be [n, dim], not {tuple(table.shape)}")
+    _no_grad("table", table)
     dev, bits, kind = _cuda(table, ids), _id_bits(ids), _type_id(table.dtype)
     n, dim = table.shape
     ctx, index, st = _enter(dev, stream, table, ids)
@@ -244,6 +254,7 @@ def rows_grad_device(grad_out: torch.Tensor, ids: torch.Tensor, n_rows: int, sca
     dim = grad_out.shape[-1]
     if tuple(grad_out.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"grad_out {tuple(grad_out.shape)} does not fit ids {tuple(ids.shape)}")
+    _no_grad("grad_out", grad_out)
     given = (grad_out, ids) if out is None else (grad_out, ids, out)
     dev, bits, kind = _cuda(*given), _id_bits(ids), _type_id(grad_out.dtype)
     out_dtype = out.dtype if out is not None else dtype or grad_out.dtype

@@ -47,3 +47,12 @@ def test_a_trained_table(gpu):
     assert bool((abs(weight.grad.double().cpu().numpy() - want) <= (cnt[:, None] + 1) * 2.0 ** -24 * mag * 1.001 + 1e-45).all())
     with torch.no_grad():
         assert torch.equal(R.rows_lookup_device(weight, ids, 2.0), y.detach())
+
+
+def test_a_stream_of_another_device():
+    """Neither the kernels nor the outputs' memory would be on it."""
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 0x1234
+
+    with pytest.raises(ValueError, match="a stream of cuda:1 for tensors on cuda:0"):
+        R._enter(torch.device("cuda", 0), Stream())

@@ -72,6 +72,8 @@ def _enter(dev: torch.device, stream, *inputs: torch.Tensor):
     """(context, device index, hipStream_t) for work on `dev` and `stream`: inside the context torch's copies and
     allocations belong to the stream. Inputs used on a stream that is not the current one are kept for it."""
     index = dev.index if dev.index is not None else torch.cuda.current_device()
+    if stream is not None and stream.device.index != index:
+        raise ValueError(f"a stream of {stream.device} for tensors on {dev}")
     if stream is None or stream.cuda_stream == _raw_stream(index):
         return _NO_CTX, index, _raw_stream(index)
     for t in inputs:

@@ -3022,8 +3022,12 @@ Int4Ws int4_ws(uint64_t n, uint32_t dim, uint32_t nq, uint32_t k) {
         }
         // k of a sample of S rows bound about k n / S of all. A block finds the bound of a query in S / 1200 us and the
         // collection takes 0.2 us per 1000 candidates: their sum is least at `expect` candidates per query (100 queries,
-        // k = 10: 1M x 128 with 512 178 us and with 2048 195; 10M x 128 3046 and 2228). The bound scatters (by a gamma
-        // distribution of shape k), and the collection's room is not to run out by chance: odds under 1e-6 per query.
+        // k = 10: 1M x 128 with 512 178 us and with 2048 195; 10M x 128 3046 and 2228). The bound scatters, for rows in an
+        // order that has nothing to do with their values by a gamma distribution of shape k: the odds that the collection's
+        // room runs out are then under 1e-6 per query. The sample takes whole tiles, so where neighbouring rows are alike
+        // sixteen of them count as little more than one, the shape is nearer to k / 16, and some queries of a batch
+        // overflow: the levels answer, at the price of a second pass (10M x 128, 100 queries, k = 10: 1260 us in random
+        // order, 4050 to 5200 with runs of 16 to 256 alike rows; 1M x 128: 190 and 180 to 200).
         // At most a sixteenth of the rows, but no fewer than expect half of that room to be filled.
         const uint64_t kn = (uint64_t)k * n;
         const double nq_ = (double)std::max<uint64_t>(qc, 1), least = std::sqrt((double)kn * std::ceil(nq_ / 256) / (0.24 * nq_));

@@ -429,7 +429,7 @@ __device__ __forceinline__ void int4_block_digits(const TQ *queries, uint32_t nq
 
 // The running sum of one (row, query) pair gains one group: c = the integer products of the four digits, put together
 // exactly (42 bits), times the group's scale. In f64 throughout: an f32 part for the lower digits would overflow where rows
-// are large, and measured no faster (1M x 960, 64 queries: 476 us against 500).
+// are large, and measured no faster.
 __device__ __forceinline__ double int4_add(double acc, i32x4_t c, double s) {
     return __builtin_fma(s, __builtin_fma((double)(c[2] + (c[3] << 8)), 65536.0, (double)(c[0] + (c[1] << 8))), acc);
 }
@@ -1003,7 +1003,8 @@ __device__ __forceinline__ void grad_store(O *o, const float (&sum)[V], float sc
 // The sums. The sorted places are cut into chunks of R; L = 1 << lg lanes take one chunk and L * V columns, V columns a
 // lane, and walk the chunk with the rows of U places in flight. A run that lies inside the chunk goes to the gradient;
 // of a run that the chunk's borders cut, the part that opens the run goes to part[2c + 1], a part that continues one to
-// part[2c] (f32, dim columns), and rows_grad_join_kernel adds them up. So no run, however long, is one wave's work.
+// part[2c] (f32, dim columns), and rows_grad_join_kernel adds them up. So no run, however long, is summed by one wave; its parts are joined by
+// one block per 64 * V columns.
 // Blocks from `blocks` on zero the rows that no id names. Bound by the read of the gradients, a row at a time, and the
 // write of the table's gradient.
 struct GradArgs {

@@ -15,8 +15,8 @@ constexpr uint32_t int4_gstride(uint32_t dim, uint32_t group) {
     return (groups + m - 1) / m * m;
 }
 
-// Threads. Five and eight quartets of one tile: sixteen waves around one copy of the digits (1M x 960, 64 queries: 472 us,
-// 496 with eight waves of two tiles each; 20 queries: 196 and 215).
+// Threads. Five and eight quartets of one tile: sixteen waves around one copy of the digits (1M x 960, 64 queries: 431 us,
+// 625 with eight waves of two tiles each; 20 queries: 207 and 252).
 constexpr int int4_block(int qt, int t) { return qt >= 5 && t == 1 ? 1024 : qt >= 3 ? 512 : 256; }
 
 constexpr uint32_t int4_lds_kb(int qt) { return qt >= 5 ? 128u : qt >= 3 ? 144u : 64u; } // digits per block: one large block per CU, or several

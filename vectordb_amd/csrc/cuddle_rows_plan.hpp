@@ -40,8 +40,9 @@ constexpr uint32_t int4_scales(int p, uint32_t group) { return (uint32_t)p * 64 
 // Rows of one or two units have one pair of units to request ahead, and their scales are too few for more (int4_scales).
 // Five quartets then take two tiles, which keeps the wave busy (1M x 128, 100 queries: 245 us against 295; from 192
 // dimensions on equal or slower, 100k x 4096: 455 against 345); with eight, two tiles do not fit the registers. Eight
-// against five for such rows (1M x 128, search, k = 10): 64 queries 132 us and 137, 128 207 and 221, 200 345 and 308, 1000
-// 1200 and 1560; distances, bound by their own writes, 267 and 290 at 101, 345 and 334 at 128.
+// against five for such rows (1M x 128; search, k = 10: 64 queries 132 us and 137, 128 207 and 221, 200 345 and 308, 1000
+// 1200 and 1560; distances, mostly their own writes, 267 and 290 at 101, 345 and 334 at 128, 522 and 445 at 200). The rule is
+// kept the same for all rows; 160 to 200 queries are where it loses on such short ones.
 struct Int4Shape {
     int qt, t, p;
 };
